@@ -36,6 +36,10 @@ GT_ERR_NCCL = -6
 GT_ERR_TOO_LARGE = -7
 GT_ERR_NOT_INIT = -8
 
+# what becomes of the rows' losses
+REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+TOP_MAX = 1024           # teacher logits per row that the distillation losses take
+
 _F = POINTER(c_float)
 
 # name -> (restype, argtypes); mirrors include/gt_b200.h declaration by declaration
@@ -136,6 +140,15 @@ SIGNATURES = {
                                        c_int64, c_int64, c_int, c_float]),
     "gt_cross_entropy_backward": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_float,
                                           c_int64, c_int64, c_int]),
+    "gt_linear_loss_sizes": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, POINTER(c_size_t), POINTER(c_size_t)]),
+    "gt_linear_cross_entropy": (c_int, [c_void_p] + [c_void_p] * 6 + [c_int64] * 3 + [c_float, c_int, c_int]),
+    "gt_linear_topk_distillation": (c_int, [c_void_p] + [c_void_p] * 7 + [c_int64] * 4 + [c_float, c_int, c_int]),
+    "gt_linear_loss_backward": (c_int, [c_void_p] + [c_void_p] * 7 + [c_int64] * 4 + [c_float, c_int, c_int, c_int, c_int]),
+    "gt_topk_distillation_sizes": (c_int, [c_void_p, c_int64, c_int64, c_int64, POINTER(c_size_t)]),
+    "gt_topk_distillation": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64,
+                                     c_float, c_int]),
+    "gt_topk_distillation_backward": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64,
+                                              c_float, c_int, c_int]),
     "gt_adamw": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_float, c_float, c_float, c_float,
                          c_float, c_float, c_float, c_void_p]),
     "gt_sumsq": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int]),

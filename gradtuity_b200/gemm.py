@@ -25,6 +25,15 @@ def default_precision() -> int:
     return _PRECISIONS[name]
 
 
+def precision_of(name: str | None) -> int:
+    """The code of a precision given by name; None is the default precision."""
+    if name is None:
+        return default_precision()
+    if name not in _PRECISIONS:
+        raise ValueError(f"precision must be one of {sorted(_PRECISIONS)}, got {name!r}")
+    return _PRECISIONS[name]
+
+
 def _p(x):
     return c_void_p(x) if x else None
 

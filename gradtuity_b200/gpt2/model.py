@@ -68,14 +68,25 @@ class GPT2Small(Module):
         self.ln_f = LayerNorm(n_embd)
         self.lm_head = TiedLMHead(self.wte)
 
-    def __call__(self, input_ids: Tensor) -> Tensor:
+    def hidden(self, input_ids: Tensor) -> Tensor:
+        """The hidden states (B, S, n_embd) that the head reads."""
         B, S = input_ids.shape
         x = self.wte(input_ids).add(self.wpe(seq_len=S, batch_size=B, start_pos=0))
         x = self.drop(x)
         for block in self.blocks:
             x = block(x)
-        x = self.ln_f(x)
-        return self.lm_head(x)
+        return self.ln_f(x)
+
+    def __call__(self, input_ids: Tensor) -> Tensor:
+        return self.lm_head(self.hidden(input_ids))
+
+    def loss(self, input_ids: Tensor, labels: Tensor, ignore_index: int = -100) -> Tensor:
+        """Mean cross entropy against labels (B * S,), the logits never kept (TiedLMHead.cross_entropy)."""
+        return self.lm_head.cross_entropy(self.hidden(input_ids), labels, ignore_index=ignore_index)
+
+    def distillation_loss(self, input_ids: Tensor, teacher_ids: Tensor, teacher_logits: Tensor, temperature: float = 1.0) -> Tensor:
+        """Mean distillation loss against a teacher's top logits, (B * S, top) each (TiedLMHead.topk_distillation)."""
+        return self.lm_head.topk_distillation(self.hidden(input_ids), teacher_ids, teacher_logits, temperature=temperature)
 
     def parameters(self) -> list[Tensor]:
         params = []

@@ -204,6 +204,22 @@ class TiedLMHead(Module):
         logits = h.view((B * S, E)).linear_tied(wte.weight)
         return logits.view((B, S, wte.num_embeddings))
 
+    def _tokens(self, h: Tensor) -> Tensor:
+        E = h.shape[-1]
+        if E != self.embedding_module.embedding_dim:
+            raise ValueError(f"input last dim {E} must equal embedding_dim {self.embedding_module.embedding_dim}")
+        return h.view((-1, E))
+
+    def cross_entropy(self, h: Tensor, targets: Tensor, reduction: str = "mean", ignore_index: int = -100) -> Tensor:
+        """The cross entropy of this head's logits against `targets` (B * S,), without the logits
+        (`Tensor.linear_cross_entropy`)."""
+        return self._tokens(h).linear_cross_entropy(self.weight_ref, targets, reduction=reduction, ignore_index=ignore_index)
+
+    def topk_distillation(self, h: Tensor, teacher_ids: Tensor, teacher_logits: Tensor, temperature: float = 1.0, reduction: str = "mean") -> Tensor:
+        """Distillation of this head's logits from a teacher's top logits, (B * S, top) each, without the logits
+        (`Tensor.linear_topk_distillation`)."""
+        return self._tokens(h).linear_topk_distillation(self.weight_ref, teacher_ids, teacher_logits, temperature=temperature, reduction=reduction)
+
     def parameters(self) -> list[Tensor]:
         return []
 

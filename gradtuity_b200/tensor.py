@@ -22,7 +22,7 @@ import math
 import os
 import struct
 from contextlib import contextmanager
-from ctypes import c_void_p
+from ctypes import byref, c_size_t, c_void_p
 from typing import Callable, Optional
 
 from . import _lib
@@ -1181,6 +1181,116 @@ class Tensor:
                       _vp(g.ptr), (1.0 / Bn) if reduction == "mean" else 1.0, Bn, C, 0 if fresh else 1)
 
         out._set_graph(parents=(self, targets), backward_fn=_backward)
+        return out
+
+    # ---- losses of the language-model head ------------------------------------------------------
+
+    @staticmethod
+    def _loss_checks(opname: str, reduction: str, temperature: float = 1.0) -> int:
+        if reduction not in _lib.REDUCTIONS:
+            raise ValueError(f"{opname} reduction must be 'none', 'mean' or 'sum', got {reduction!r}")
+        if not (temperature > 0.0 and math.isfinite(temperature)):
+            raise ValueError(f"{opname} temperature must be positive and finite, got {temperature}")
+        return _lib.REDUCTIONS[reduction]
+
+    @staticmethod
+    def _teacher_checks(opname: str, rows: int, ids: "Tensor", teacher: "Tensor") -> int:
+        if ids.ndim != 2 or teacher.shape != ids.shape:
+            raise ValueError(f"{opname} expects teacher ids and logits of one (rows, top) shape, got {ids.shape} and {teacher.shape}")
+        if ids.shape[0] != rows:
+            raise ValueError(f"{opname} batch size mismatch: {rows} rows vs {ids.shape[0]} of the teacher")
+        if ids.shape[1] > _lib.TOP_MAX:
+            raise ValueError(f"{opname} takes at most {_lib.TOP_MAX} teacher logits per row, got {ids.shape[1]}")
+        return ids.shape[1]
+
+    def _linear_loss(self, opname: str, entry: str, weight: "Tensor", given: tuple["Tensor", ...], top: int, temperature: float, extra: tuple,
+                     reduction: int, precision: str | None) -> "Tensor":
+        if self.ndim != 2:
+            raise ValueError(f"{opname} requires 2D input, got shape {self._shape}")
+        if weight.ndim != 2:
+            raise ValueError(f"weight must be 2D, got shape {weight._shape}")
+        if self._shape[1] != weight._shape[1]:
+            raise ValueError(f"{opname} shape mismatch: input last dim {self._shape[1]} != weight last dim {weight._shape[1]}")
+        prec = _gemm.precision_of(precision)
+        M, E = self._shape
+        V, _ = weight._shape
+        n_saved, n_scratch = c_size_t(0), c_size_t(0)
+        _call("gt_linear_loss_sizes", M, V, E, top, prec, byref(n_saved), byref(n_scratch))
+        saved = alloc_storage(n_saved.value)
+        out = empty_tensor((M,) if reduction == _lib.REDUCTIONS["none"] else (1,))
+        with temp_storage(n_scratch.value) as scratch:
+            _call(entry, _vp(out.ptr), _vp(saved.ptr), _vp(scratch.ptr), _vp(self.ptr), _vp(weight.ptr), *(_vp(t.ptr) for t in given), M, V, E,
+                  *extra, reduction, prec)
+        x = self
+
+        def _backward(g: "Tensor") -> None:
+            dx, acc_dx = grad_target(x) if x.requires_grad else (0, False)
+            dw, acc_dw = grad_target(weight) if weight.requires_grad else (0, False)
+            with temp_storage(n_scratch.value) as scratch:
+                _call("gt_linear_loss_backward", _vp(dx), _vp(dw), _vp(saved.ptr), _vp(scratch.ptr), _vp(x.ptr), _vp(weight.ptr), _vp(g.ptr),
+                      M, V, E, top, temperature, reduction, prec, int(acc_dx), int(acc_dw))
+
+        out._set_graph(parents=(self, weight), backward_fn=_backward)
+        return out
+
+    def linear_cross_entropy(self, weight: "Tensor", targets: "Tensor", reduction: str = "mean", ignore_index: int = -100,
+                             precision: str | None = None) -> "Tensor":
+        """`self.linear_tied(weight).cross_entropy(targets)` without the (rows, words) logits: self (M, E) hidden states,
+        weight (V, E), targets (M,) float-encoded ids.  The logits are computed in pieces of the vocabulary, forward and
+        again backward, and never kept.
+
+        Rows whose target is `ignore_index` have no loss and no gradient and do not count in the mean, which is 0 when no row
+        counts.  `reduction` is 'none' (the rows' losses, (M,)), 'mean' or 'sum' ((1,)).  `precision` is that of the products,
+        'tf32', '3xtf32' or 'fp32' (the last two are as exact as sums in 32 bits); by default the one of the GEMMs
+        (GRADTUITY_GEMM_PRECISION).  A target outside the vocabulary is reported by the device status word."""
+        mode = self._loss_checks("linear_cross_entropy", reduction)
+        if targets.ndim != 1:
+            raise ValueError(f"linear_cross_entropy expects 1D targets, got ndim={targets.ndim}")
+        if self.ndim == 2 and targets.shape[0] != self._shape[0]:
+            raise ValueError(f"linear_cross_entropy batch size mismatch: input {self._shape[0]} vs targets {targets.shape[0]}")
+        return self._linear_loss("linear_cross_entropy", "gt_linear_cross_entropy", weight, (targets,), 1, 1.0, (float(ignore_index),), mode, precision)
+
+    def linear_topk_distillation(self, weight: "Tensor", teacher_ids: "Tensor", teacher_logits: "Tensor", temperature: float = 1.0,
+                                 reduction: str = "mean", precision: str | None = None) -> "Tensor":
+        """`self.linear_tied(weight).topk_distillation(teacher_ids, teacher_logits, ...)` without the (rows, words) logits, in
+        pieces of the vocabulary as `linear_cross_entropy`."""
+        mode = self._loss_checks("linear_topk_distillation", reduction, temperature)
+        top = self._teacher_checks("linear_topk_distillation", self._shape[0], teacher_ids, teacher_logits)
+        return self._linear_loss("linear_topk_distillation", "gt_linear_topk_distillation", weight, (teacher_ids, teacher_logits), top,
+                                 float(temperature), (top, float(temperature)), mode, precision)
+
+    def topk_distillation(self, teacher_ids: "Tensor", teacher_logits: "Tensor", temperature: float = 1.0, reduction: str = "mean") -> "Tensor":
+        """Distillation of (B, C) logits from a teacher's top logits: T^2 KL(q || softmax(self / T)) per row, where q is the
+        softmax of the teacher's logits / T over the row's entries in use.  teacher_ids (float-encoded) and teacher_logits are
+        (B, top), top <= 1024, in any order; an entry with a negative id, or a logit of -inf or NaN, is not in use; an id that
+        comes twice adds up.  A row without any entry in use has no loss and no gradient and does not count in the mean.
+        `reduction` as in `linear_cross_entropy`."""
+        mode = self._loss_checks("topk_distillation", reduction, temperature)
+        if self.ndim != 2:
+            raise ValueError(f"topk_distillation expects 2D logits, got ndim={self.ndim}")
+        Bn, C = self._shape
+        top = self._teacher_checks("topk_distillation", Bn, teacher_ids, teacher_logits)
+        n_saved = c_size_t(0)
+        _call("gt_topk_distillation_sizes", Bn, C, top, byref(n_saved))
+        saved = alloc_storage(n_saved.value)
+        out = empty_tensor((Bn,) if reduction == "none" else (1,))
+        x_ptr, x_ld = self._rows()
+        T = float(temperature)
+        _call("gt_topk_distillation", _vp(out.ptr), _vp(saved.ptr), _vp(x_ptr), x_ld, _vp(teacher_ids.ptr), _vp(teacher_logits.ptr), Bn, C, top, T, mode)
+        logits = self
+
+        def _backward(g: "Tensor") -> None:
+            if not logits.requires_grad:
+                return
+            fresh = logits.grad is None
+            if fresh:
+                # written, not accumulated; padded like the logits so that the products behind them read it by TMA
+                logits.grad = empty_padded_tensor(logits.shape, logits._rows()[1])
+            d_ptr, d_ld = logits.grad._rows()
+            lx_ptr, lx_ld = logits._rows()
+            _call("gt_topk_distillation_backward", _vp(d_ptr), d_ld, _vp(saved.ptr), _vp(lx_ptr), lx_ld, _vp(g.ptr), Bn, C, top, T, mode, 0 if fresh else 1)
+
+        out._set_graph(parents=(self,), backward_fn=_backward)
         return out
 
     def conv2d(self, weight: "Tensor", bias: "Tensor", stride: int = 1, padding: int = 0) -> "Tensor":

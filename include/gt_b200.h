@@ -386,6 +386,45 @@ int gt_cross_entropy_fused(gt_ctx* ctx, float* loss, float* row_loss, float* row
 int gt_cross_entropy_backward(gt_ctx* ctx, float* dlogits, int64_t ld_dlogits, const float* logits,
                               int64_t ld_logits, const float* targets, const float* row_lse,
                               const float* upstream, float scale, int64_t B, int64_t C, int accumulate);
+
+/* ---- losses of the language-model head (no counterpart in the reference, which composes linear_tied and cross_entropy,
+ *      gradtuity/tensor.py:1452-1525, 1684-1779, and has no distillation loss) -------------------------------------------
+ * Sparse targets: row t has (id, q) pairs.  Cross entropy has one pair with q = 1 (none where targets[t] == ignore_index).
+ * Distillation takes the teacher's top logits: ids and teacher are (M, K), K <= 1024, in any order, an id may repeat; an entry
+ * is in use when its id is >= 0 and its logit is above -inf (a NaN logit is not in use); q = softmax(teacher / T) over the
+ * entries in use.  A row with no target in use has no loss and no gradient and does not count.  With z = logits / T,
+ *     loss_t = T^2 sum_k q_tk (log q_tk - log softmax(z_t)[id_tk]),   d loss_t / d logits_t = T (softmax(z_t) - q_t)
+ * loss receives M values (GT_REDUCE_NONE) or one: their sum, or their mean over the rows that count (0 when none does).
+ * ids are float-encoded (V < 2^24); one that is in use and >= V, or a target outside [0, V) other than ignore_index, sets the
+ * status word to GT_ERR_INVALID_ARG and is left out.  All on the context's compute stream; x (M, E), w (V, E), no padding.
+ *
+ * The linear forms take hidden states x and the vocabulary matrix w; the logits are x w^T, computed in pieces of the
+ * vocabulary and never kept.  precision: GT_PREC_TF32 rounds the operands of the products to 11 bits; GT_PREC_TF32X3 and
+ * GT_PREC_FP32 are as exact as sums in 32 bits.  `saved` is what the forward pass leaves for the backward pass, `scratch` is free
+ * for other use once the call's work is done; gt_linear_loss_sizes gives the bytes of both (256-byte aligned, both not NULL;
+ * K = 1 for cross entropy).  gt_linear_loss_backward serves both losses: T = 1, K = 1 for cross entropy; the other arguments as
+ * in the forward call.  upstream: the gradient of the loss, on the device: M values for GT_REDUCE_NONE, else one.  dx or dw
+ * may be NULL; acc_* adds to the buffer instead of overwriting it.                                                     */
+#define GT_REDUCE_NONE 0
+#define GT_REDUCE_MEAN 1
+#define GT_REDUCE_SUM  2
+int gt_linear_loss_sizes(gt_ctx* ctx, int64_t M, int64_t V, int64_t E, int64_t K, int precision, size_t* saved, size_t* scratch);
+int gt_linear_cross_entropy(gt_ctx* ctx, float* loss, void* saved, void* scratch, const float* x, const float* w, const float* targets,
+                            int64_t M, int64_t V, int64_t E, float ignore_index, int reduction, int precision);
+int gt_linear_topk_distillation(gt_ctx* ctx, float* loss, void* saved, void* scratch, const float* x, const float* w, const float* ids,
+                                const float* teacher, int64_t M, int64_t V, int64_t E, int64_t K, float temperature, int reduction,
+                                int precision);
+int gt_linear_loss_backward(gt_ctx* ctx, float* dx, float* dw, void* saved, void* scratch, const float* x, const float* w,
+                            const float* upstream, int64_t M, int64_t V, int64_t E, int64_t K, float temperature, int reduction,
+                            int precision, int acc_dx, int acc_dw);
+/* Distillation on given logits (B, C), rows ld floats apart.  saved: gt_topk_distillation_sizes bytes.                  */
+int gt_topk_distillation_sizes(gt_ctx* ctx, int64_t B, int64_t C, int64_t K, size_t* saved);
+int gt_topk_distillation(gt_ctx* ctx, float* loss, void* saved, const float* logits, int64_t ld_logits, const float* ids,
+                         const float* teacher, int64_t B, int64_t C, int64_t K, float temperature, int reduction);
+int gt_topk_distillation_backward(gt_ctx* ctx, float* dlogits, int64_t ld_dlogits, void* saved, const float* logits, int64_t ld_logits,
+                                  const float* upstream, int64_t B, int64_t C, int64_t K, float temperature, int reduction,
+                                  int accumulate);
+
 int gt_adamw(gt_ctx* ctx, float* p, const float* g, float* m, float* v, int64_t n, float lr, float beta1,
              float beta2, float eps, float weight_decay, float bc1, float bc2, const float* grad_scale);
 int gt_sumsq(gt_ctx* ctx, float* out, const float* x, int64_t n, int accumulate);
