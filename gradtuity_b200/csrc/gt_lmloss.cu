@@ -8,19 +8,22 @@
 // the teacher's top logits / T over the entries in use.  A row without any target in use has weight 0: no loss, no gradient.
 // m and s are kept apart instead of as m + log s: p then carries no rounding of a sum of that size.
 //
-// Linear forms: the (tokens x words) logits are never kept.  Both directions walk over pieces of the vocabulary; the backward
-// computes a piece's logits again, turns them into the logits' gradient G in place, and multiplies:
-//     dx += G W_piece,   dW_piece = G^T x.
+// Linear forms: the (tokens x words) logits are never kept.  The forward pass keeps each row's m and s, the backward pass walks
+// over pieces of the vocabulary, computes a piece's logits again, turns them into the logits' gradient G, and multiplies:
+//     dx += G W_piece,   dW_piece = G^T x      (gt_lmloss_umma.cu)
+// Rows that do not count are left out from the start: the products work on the others, closed up ("compact" rows).
 
 #include <math.h>
 
-#include "gt_internal.h"
+#include <cuda_fp16.h>
+
+#include "gt_lmloss.h"
 
 namespace {
 
 constexpr int TOP_MAX = 1024;                       // targets of a row: they are sorted in shared memory
 constexpr int UNUSED = 0x7fffffff;                  // id of a place that is not in use; sorts behind every word
-constexpr long long PIECE_BYTES = 64ll << 20;       // what one piece of logits may occupy
+constexpr long long PIECE_BYTES = 64ll << 20;       // what G of one piece of the vocabulary may occupy
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -55,35 +58,44 @@ __device__ __forceinline__ MaxSum warp_join(MaxSum a) {
 
 // What the forward pass leaves for the backward pass, in one block of memory.
 struct Saved {
-  int* count;       // rows that count
-  float2* stats;    // (m, s) per row
-  float* weight;    // 1, or 0 for a row that does not count
-  float* konst;     // sum of q log q per row
+  LmScalars* scalars;
+  float* weight;    // by row: 1, or 0 for a row that does not count
+  float* konst;     // by row: sum of q log q
   int* ids;         // (M, K), ascending, UNUSED at the end
   float* q;         // (M, K), 0 where unused
+  int* row_of;      // rows that count, in order
+  float2* stats;    // by row (distillation of given logits), or by compact row and with m in units of log 2 (linear forms)
+  float2* factor;   // by compact row, see LmProblem
   size_t bytes;
 };
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
-Saved saved_layout(void* base, long long M, long long K) {
+struct Carve {
+  char* p; size_t at;
+  template <class T> T* take(size_t n) { T* r = (T*)(p + at); at += up256(n * sizeof(T)); return r; }
+};
+Saved saved_layout(Carve& c, long long M, long long K) {
   Saved s;
-  char* p = (char*)base;
-  size_t at = 0;
-  auto take = [&](size_t n) { char* r = p + at; at += up256(n); return r; };
-  s.count = (int*)take(sizeof(int));
-  s.stats = (float2*)take(sizeof(float2) * M);
-  s.weight = (float*)take(sizeof(float) * M);
-  s.konst = (float*)take(sizeof(float) * M);
-  s.ids = (int*)take(sizeof(int) * M * K);
-  s.q = (float*)take(sizeof(float) * M * K);
-  s.bytes = at;
+  s.scalars = c.take<LmScalars>(1);
+  s.weight = c.take<float>(M);
+  s.konst = c.take<float>(M);
+  s.ids = c.take<int>(M * K);
+  s.q = c.take<float>(M * K);
+  s.row_of = c.take<int>(M);
+  s.stats = c.take<float2>(M);
+  s.factor = c.take<float2>(M);
+  s.bytes = c.at;
   return s;
+}
+Saved saved_layout(void* base, long long M, long long K) {
+  Carve c = {(char*)base, 0};
+  return saved_layout(c, M, K);
 }
 
 // ---- targets -------------------------------------------------------------------------------------
 
 // Cross entropy: one target of q = 1 per row.  An id outside the vocabulary sets the status word.
 __global__ void __launch_bounds__(256) hard_targets_kernel(const float* __restrict__ targets, long long M, long long V, float ignore,
-                                                           Saved s, int* status) {
+                                                           Saved s, float* __restrict__ row_loss, int* status) {
   const long long t = (long long)blockIdx.x * blockDim.x + threadIdx.x;
   bool used = false;
   if (t < M) {
@@ -95,24 +107,24 @@ __global__ void __launch_bounds__(256) hard_targets_kernel(const float* __restri
     s.q[t] = used ? 1.0f : 0.0f;
     s.weight[t] = used ? 1.0f : 0.0f;
     s.konst[t] = 0.0f;
+    if (!used) row_loss[t] = 0.0f;
   }
-  const int n = __syncthreads_count(used);
-  if (threadIdx.x == 0 && n) atomicAdd(s.count, n);        // whole numbers: the order does not matter
 }
 
 // Distillation: a warp per row.  q = softmax(teacher / T) over the places in use (id >= 0, logit above -inf), sorted by id by
 // counting, for each place, the places that go before it (K^2 comparisons, K is tens to a few hundred).
 __global__ void __launch_bounds__(128) top_targets_kernel(const float* __restrict__ ids, const float* __restrict__ teacher, long long M,
-                                                          long long V, int K, float inv_T, Saved s, int* status) {
+                                                          long long V, int K, float inv_T, Saved s,
+                                                          float* __restrict__ row_loss, int* status) {
   extern __shared__ float smem[];
   const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
   int* key = reinterpret_cast<int*>(smem) + (size_t)w * 2 * K;
   float* val = reinterpret_cast<float*>(key + K);
-  __shared__ int counted[4];
   const long long t = (long long)blockIdx.x * 4 + w;
   float mx = -INFINITY;
   bool any = false;
-  if (t < M) {
+  if (t >= M) return;
+  {
     for (int k = l; k < K; k += 32) {
       const float f = ids[t * K + k], v = teacher[t * K + k];
       bool used = !(f < 0.0f) && v > -INFINITY;
@@ -147,21 +159,135 @@ __global__ void __launch_bounds__(128) top_targets_kernel(const float* __restric
       s.q[t * K + before] = q;
     }
     konst = warp_sum(konst);
-    if (l == 0) { s.weight[t] = any ? 1.0f : 0.0f; s.konst[t] = konst; }
+    if (l == 0) {
+      s.weight[t] = any ? 1.0f : 0.0f;
+      s.konst[t] = konst;
+      if (!any) row_loss[t] = 0.0f;
+    }
   }
-  if (l == 0) counted[w] = any;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    const int n = counted[0] + counted[1] + counted[2] + counted[3];
-    if (n) atomicAdd(s.count, n);
+}
+
+// row_of: the rows that count, in order; count: how many.  One block.
+__global__ void __launch_bounds__(1024) compact_rows_kernel(long long M, Saved s) {
+  __shared__ int sums[32];
+  const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
+  int base = 0;
+  for (long long t0 = 0; t0 < M; t0 += 1024) {
+    const long long t = t0 + threadIdx.x;
+    const bool counts = t < M && s.weight[t] != 0.0f;
+    const unsigned mask = __ballot_sync(0xffffffffu, counts);
+    if (l == 0) sums[w] = __popc(mask);
+    __syncthreads();
+    const int mine = sums[l];
+    int before = w > l ? mine : 0, all = mine;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      before += __shfl_xor_sync(0xffffffffu, before, o);
+      all += __shfl_xor_sync(0xffffffffu, all, o);
+    }
+    if (counts) s.row_of[base + before + __popc(mask & ((1u << l) - 1))] = (int)t;
+    base += all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) s.scalars->count = base;
+}
+
+// ---- operands of the linear forms: largest value, then the split into halves ------------------------
+
+// Whole matrix w, and of x the rows that count.  A maximum of bits as whole numbers, so the order of the additions is no matter.
+__global__ void __launch_bounds__(256) largest_kernel(const float* __restrict__ x, const float* __restrict__ w, long long V, long long E, Saved s,
+                                                      int blocks_x) {
+  const bool is_x = (int)blockIdx.x < blocks_x;
+  const long long rows = is_x ? s.scalars->count : V;
+  const int first = is_x ? blockIdx.x : blockIdx.x - blocks_x, step = is_x ? blocks_x : gridDim.x - blocks_x;
+  const float* src = is_x ? x : w;
+  const bool vec = ((uintptr_t)src & 15) == 0 && E % 4 == 0;
+  unsigned m = 0;
+  auto see = [&](float f) {
+    const unsigned b = __float_as_uint(f) & 0x7fffffffu;
+    if (b < 0x7f800000u && b > m) m = b;                     // infinities and NaN do not set the scale
+  };
+  if (!is_x && vec) {
+    const float4* p = reinterpret_cast<const float4*>(src);
+    const long long n = rows * E / 4;
+    long long i = (long long)first * 256 + threadIdx.x;
+    for (; i + 3ll * step * 256 < n; i += 4ll * step * 256) {
+      float4 a[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) a[k] = p[i + (long long)k * step * 256];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) { see(a[k].x); see(a[k].y); see(a[k].z); see(a[k].w); }
+    }
+    for (; i < n; i += (long long)step * 256) { const float4 a = p[i]; see(a.x); see(a.y); see(a.z); see(a.w); }
+  } else {
+    for (long long r = (long long)first * 8 + (threadIdx.x >> 5); r < rows; r += (long long)step * 8) {
+      const float* p = src + (is_x ? s.row_of[r] : r) * E;
+      for (long long e = threadIdx.x & 31; e < E; e += 32) see(p[e]);
+    }
+  }
+  m = __reduce_max_sync(0xffffffffu, m);
+  if ((threadIdx.x & 31) == 0 && m) atomicMax(is_x ? &s.scalars->amax_x : &s.scalars->amax_w, m);
+}
+
+// v = 2^e (scaled value), the largest scaled value in [2^14, 2^15): fp16 holds it, and halves down to 2^-24 of an ulp each
+__device__ __forceinline__ int scale_exponent(unsigned amax) {
+  if (amax == 0) return 0;
+  const int e = (int)(amax >> 23) - 127;
+  return (e < -100 ? -100 : e) - 14;
+}
+
+// A warp per row.  x: compact rows, and zeros behind them to the end of the last tile of rows.
+__global__ void __launch_bounds__(256) split_kernel(const float* __restrict__ x, const float* __restrict__ w, long long M, long long V, long long E,
+                                                    long long pitch, Saved s, LmSplit xs, LmSplit ws, int products, float T, int blocks_x) {
+  const int l = threadIdx.x & 31;
+  const bool is_x = (int)blockIdx.x < blocks_x;
+  const int ex = scale_exponent(s.scalars->amax_x), ew = scale_exponent(s.scalars->amax_w);
+  if (blockIdx.x == 0 && threadIdx.x == 0) s.scalars->logit2 = ldexpf(1.4426950408889634f / T, ex + ew);
+  const long long count = s.scalars->count;
+  const long long up_to = (count + LM_TILE - 1) / LM_TILE * LM_TILE;
+  const long long rows = is_x ? (up_to < M ? up_to : M) : V;
+  const int first = is_x ? blockIdx.x : blockIdx.x - blocks_x, step = is_x ? blocks_x : gridDim.x - blocks_x;
+  const float scale = ldexpf(1.0f, -(is_x ? ex : ew));
+  const LmSplit d = is_x ? xs : ws;
+  const bool vec = ((uintptr_t)(is_x ? x : w) & 15) == 0 && E % 4 == 0;
+  auto halves = [&](float v, unsigned short& hi, unsigned short& lo) {
+    const float f = v * scale;
+    const __half h = __float2half_rn(f);
+    hi = __half_as_ushort(h);
+    lo = __half_as_ushort(__float2half_rn(f - __half2float(h)));
+  };
+  for (long long i = (long long)first * 8 + (threadIdx.x >> 5); i < rows; i += (long long)step * 8) {
+    // w from its end: the tail of it is still in L2 from the pass before
+    const long long r = is_x ? i : rows - 1 - i;
+    const bool zero = is_x && r >= count;
+    const float* src = is_x ? x + (zero ? 0ll : (long long)s.row_of[r]) * E : w + r * E;
+    uint16_t* hi = d.hi + r * pitch;
+    uint16_t* lo = d.lo + r * pitch;
+    if (vec) {
+#pragma unroll 4
+      for (long long e = 4 * l; e < E; e += 128) {
+        const float4 a = zero ? make_float4(0.f, 0.f, 0.f, 0.f) : *reinterpret_cast<const float4*>(src + e);
+        ushort4 h, o;
+        halves(a.x, h.x, o.x); halves(a.y, h.y, o.y); halves(a.z, h.z, o.z); halves(a.w, h.w, o.w);
+        *reinterpret_cast<ushort4*>(hi + e) = h;
+        if (products == 3) *reinterpret_cast<ushort4*>(lo + e) = o;
+      }
+    } else {
+      for (long long e = l; e < E; e += 32) {
+        unsigned short h, o;
+        halves(zero ? 0.0f : src[e], h, o);
+        hi[e] = h;
+        if (products == 3) lo[e] = o;
+      }
+    }
   }
 }
 
 // ---- rows ------------------------------------------------------------------------------------------
 
-// (m, s) of a row of `n` values scaled by `scale`, joined with what `stats` holds when `carry`.  A block per row.
-__global__ void __launch_bounds__(256) row_stats_kernel(const float* __restrict__ z, long long ld, long long n, float scale, float2* __restrict__ stats,
-                                                        int carry) {
+// (m, s) of a row of `n` values scaled by `scale`.  A block per row.
+__global__ void __launch_bounds__(256) row_stats_kernel(const float* __restrict__ z, long long ld, long long n, float scale,
+                                                        float2* __restrict__ stats) {
   __shared__ MaxSum part[8];
   const long long t = blockIdx.x;
   const float* zr = z + t * ld;
@@ -175,24 +301,23 @@ __global__ void __launch_bounds__(256) row_stats_kernel(const float* __restrict_
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = a;
   __syncthreads();
   if (threadIdx.x == 0) {
-    MaxSum r = carry ? MaxSum{stats[t].x, stats[t].y} : MaxSum{-INFINITY, 0.0f};
+    MaxSum r = {-INFINITY, 0.0f};
     for (int w = 0; w < 8; ++w) r = join(r, part[w]);
     stats[t] = make_float2(r.m, r.s);
   }
 }
 
-// z -> the gradient of the loss with respect to the logits, in place or to another place: g = c (p - q), where c holds the row's
-// weight, T, the upstream gradient and 1 / n.  The columns are words [v0, v0 + n).  A block per row.
-__global__ void __launch_bounds__(256) row_grad_kernel(float* __restrict__ g, long long ld_g, const float* z, long long ld, long long v0, long long n,
-                                                       float scale, float T, Saved s, int K, const float* __restrict__ upstream, int reduction,
-                                                       int accumulate) {
+// The gradient of the loss with respect to given logits: g = c (p - q), where c holds the row's weight, T, the upstream gradient
+// and 1 / n.  A block per row.
+__global__ void __launch_bounds__(256) row_grad_kernel(float* __restrict__ g, long long ld_g, const float* z, long long ld, long long n, float scale,
+                                                       float T, Saved s, int K, const float* __restrict__ upstream, int reduction, int accumulate) {
   const long long t = blockIdx.x;
   const float* zr = z + t * ld;
   float* gr = g + t * ld_g;
   float c = s.weight[t] * T;
   if (c != 0.0f) {
     c *= reduction == GT_REDUCE_NONE ? upstream[t] : upstream[0];
-    if (reduction == GT_REDUCE_MEAN) c /= (float)*s.count;
+    if (reduction == GT_REDUCE_MEAN) c /= (float)s.scalars->count;
   }
   if (s.weight[t] == 0.0f) {
     if (!accumulate) for (long long j = threadIdx.x; j < n; j += blockDim.x) gr[j] = 0.0f;
@@ -208,27 +333,53 @@ __global__ void __launch_bounds__(256) row_grad_kernel(float* __restrict__ g, lo
   const int* ids = s.ids + t * K;
   const float* q = s.q + t * K;
   for (int k = threadIdx.x; k < K; k += blockDim.x) {
-    const long long id = ids[k];
-    if (id < v0 || id >= v0 + n || (k > 0 && ids[k - 1] == id)) continue;     // the first of a run of equal ids takes them all
+    const int id = ids[k];
+    if (id == UNUSED || (k > 0 && ids[k - 1] == id)) continue;     // the first of a run of equal ids takes them all
     float sum = 0.0f;
     for (int j = k; j < K && ids[j] == id; ++j) sum += q[j];
-    gr[id - v0] -= c * sum;
+    gr[id] -= c * sum;
   }
 }
 
-// loss_t from the row's statistics and the logits of its targets: a warp per row.  x given: logits are x_t . w_id, in fp32.
-__global__ void __launch_bounds__(256) row_loss_kernel(float* __restrict__ row_loss, const float* __restrict__ logits, long long ld,
-                                                       const float* __restrict__ x, const float* __restrict__ w, long long M, long long E, int K,
+// loss_t of given logits from the row's statistics: a warp per row.
+__global__ void __launch_bounds__(256) row_loss_kernel(float* __restrict__ row_loss, const float* __restrict__ logits, long long ld, long long M, int K,
                                                        float scale, float T, Saved s) {
   const long long t = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int l = threadIdx.x & 31;
-  if (t >= M) return;
-  if (s.weight[t] == 0.0f) {
-    if (l == 0) row_loss[t] = 0.0f;
-    return;
-  }
+  if (t >= M || s.weight[t] == 0.0f) return;
   const float2 st = s.stats[t];
   const float log_s = logf(st.y);
+  float cross = 0.0f;
+  for (int k = l; k < K; k += 32) {
+    const int id = s.ids[t * K + k];
+    if (id == UNUSED) break;
+    const float q = s.q[t * K + k];
+    if (q != 0.0f) cross += q * ((logits[t * ld + id] * scale - st.x) - log_s);
+  }
+  cross = warp_sum(cross);
+  if (l == 0) row_loss[t] = T * T * (s.konst[t] - cross);
+}
+
+// The linear forms: joins the tiles' maxima and sums of a compact row, takes the logits of its targets in 32 bits straight from
+// x and w, and writes the row's loss.  A warp per row.
+__global__ void __launch_bounds__(256) linear_row_loss_kernel(float* __restrict__ row_loss, const float2* __restrict__ partial, int parts,
+                                                              const float* __restrict__ x, const float* __restrict__ w, long long M, long long E,
+                                                              int K, float T, Saved s) {
+  const long long i = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int l = threadIdx.x & 31;
+  if (i >= s.scalars->count) return;
+  float m = -INFINITY, sum = 0.0f;                            // m in units of log 2
+  for (int j = l; j < parts; j += 32) {
+    const float2 b = partial[(long long)j * M + i];
+    const float top = fmaxf(m, b.x);
+    if (top == -INFINITY) { sum += b.y; continue; }
+    sum = sum * gt_ex2(m - top) + b.y * gt_ex2(b.x - top);
+    m = top;
+  }
+  const float top = warp_max(m);
+  sum = warp_sum(top == -INFINITY ? sum : sum * gt_ex2(m - top));
+  const long long t = s.row_of[i];
+  const float log_s = logf(sum), mean = top * 0.6931471805599453f;
   float cross = 0.0f;
   for (int k = 0; k < K; ++k) {
     const int id = s.ids[t * K + k];
@@ -236,15 +387,65 @@ __global__ void __launch_bounds__(256) row_loss_kernel(float* __restrict__ row_l
     const float q = s.q[t * K + k];
     if (q == 0.0f) continue;
     float z = 0.0f;
-    if (x) {
-      for (long long e = l; e < E; e += 32) z = fmaf(x[t * E + e], w[(long long)id * E + e], z);
-      z = warp_sum(z);
-    } else {
-      z = logits[t * ld + id];
-    }
-    cross += q * ((z * scale - st.x) - log_s);
+    for (long long e = l; e < E; e += 32) z = fmaf(x[t * E + e], w[(long long)id * E + e], z);
+    z = warp_sum(z) / T;
+    cross += q * ((z - mean) - log_s);
   }
-  if (l == 0) row_loss[t] = T * T * (s.konst[t] - cross);
+  if (l == 0) {
+    s.stats[i] = make_float2(top, sum);
+    row_loss[t] = T * T * (s.konst[t] - cross);
+  }
+}
+
+// What the rows' gradients are multiplied by.  The halves of G hold 2^14 u (p - q), u = 1, or with a gradient per row that row's
+// share of a power of two P above the largest; the rest goes into the products' own factors.  One block.
+__global__ void __launch_bounds__(1024) grad_factor_kernel(const float* __restrict__ upstream, int reduction, float T, Saved s) {
+  __shared__ unsigned part[32];
+  const int n = s.scalars->count;
+  float P = 1.0f;
+  if (reduction == GT_REDUCE_NONE) {
+    unsigned m = 0;
+    for (int i = threadIdx.x; i < n; i += 1024) {
+      const unsigned b = __float_as_uint(upstream[s.row_of[i]]) & 0x7fffffffu;
+      if (b < 0x7f800000u && b > m) m = b;
+    }
+    m = __reduce_max_sync(0xffffffffu, m);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
+    __syncthreads();
+    m = __reduce_max_sync(0xffffffffu, part[threadIdx.x & 31]);
+    if (m) { int e = (int)(m >> 23) - 126; P = ldexpf(1.0f, e < -100 ? -100 : e > 127 ? 127 : e); }
+  }
+  for (int i = threadIdx.x; i < n; i += 1024) {
+    const float u = (reduction == GT_REDUCE_NONE ? upstream[s.row_of[i]] / P : 1.0f) * 16384.0f;
+    s.factor[i] = make_float2(u / s.stats[i].y, u);
+  }
+  if (threadIdx.x == 0) {
+    float c = reduction == GT_REDUCE_NONE ? P : upstream[0];
+    if (reduction == GT_REDUCE_MEAN && n > 0) c /= (float)n;
+    c *= T;
+    s.scalars->dx = ldexpf(c, scale_exponent(s.scalars->amax_w) - 14);
+    s.scalars->dw = ldexpf(c, scale_exponent(s.scalars->amax_x) - 14);
+  }
+}
+
+// dx of rows that do not count.  A block per row.
+__global__ void __launch_bounds__(128) zero_rows_kernel(float* __restrict__ dx, long long E, Saved s) {
+  const long long t = blockIdx.x;
+  if (s.weight[t] != 0.0f) return;
+  for (long long e = threadIdx.x; e < E; e += 128) dx[t * E + e] = 0.0f;
+}
+
+// dx (+)= the shares of a piece, in order.
+__global__ void __launch_bounds__(256) add_shares_kernel(float* __restrict__ dx, const float* __restrict__ shares, int n_shares, long long M, long long E,
+                                                         int add, Saved s) {
+  const long long i = blockIdx.x;
+  if (i >= s.scalars->count) return;
+  float* to = dx + (long long)s.row_of[i] * E;
+  for (long long e = threadIdx.x; e < E; e += 256) {
+    float a = add ? to[e] : 0.0f;
+    for (int j = 0; j < n_shares; ++j) a += shares[((long long)j * M + i) * E + e];
+    to[e] = a;
+  }
 }
 
 // Sum or mean of the rows' losses in 64 bits, in a fixed order: one block.
@@ -267,81 +468,128 @@ __global__ void __launch_bounds__(1024) reduce_loss_kernel(float* __restrict__ l
 bool bad_sizes(long long M, long long V, long long K) {
   return M <= 0 || V <= 0 || K <= 0 || M > 0x7fffffff || V >= (1ll << 24) || K > TOP_MAX;    // ids are float-encoded: exact below 2^24
 }
+bool bad_width(long long E) { return E <= 0 || E > (1 << 24); }
 bool bad_temperature(float T) { return !(T > 0.0f) || isinf(T); }
 bool bad_reduction(int r) { return r != GT_REDUCE_NONE && r != GT_REDUCE_MEAN && r != GT_REDUCE_SUM; }
 
 bool bad_precision(int p) { return p != GT_PREC_TF32 && p != GT_PREC_TF32X3 && p != GT_PREC_FP32; }
 
-// words of a piece: what the byte limit allows for M rows, in whole multiples of 256
-long long piece_words(long long M, long long V) {
-  long long n = PIECE_BYTES / 4 / M / 256 * 256;
-  if (n < 256) n = 256;
-  return n < V ? n : V;
-}
-long long piece_pitch(long long words) { return (words + 3) / 4 * 4; }
+// How a linear form's work is cut up, and where everything lies.
+struct Linear {
+  Saved s;
+  LmProblem p;
+  float* row_loss;
+  int pieces;
+  size_t saved_bytes, scratch_bytes;
+};
+Linear linear_layout(gt_ctx* ctx, void* saved, void* scratch, long long M, long long V, long long E, long long K, int precision) {
+  Linear l;
+  memset(&l, 0, sizeof(l));
+  LmProblem& p = l.p;
+  p.M = M; p.V = V; p.E = E; p.K = (int)K;
+  p.products = precision == GT_PREC_TF32 ? 1 : 3;
+  p.pitch_e = (E + 7) / 8 * 8;
+  // Words of a piece: what PIECE_BYTES hold of G for M rows (two pieces of it exist at a time), in whole tiles.
+  p.words = PIECE_BYTES / 4 / M / LM_TILE * LM_TILE;
+  if (p.words < LM_TILE) p.words = LM_TILE;
+  if (p.words > V) p.words = V;
+  p.pitch_v = (p.words + 7) / 8 * 8;
+  l.pieces = (int)((V + p.words - 1) / p.words);
+  // dx has few tiles when there are few rows: its words are then shared out so that every pair of CTAs has about two units
+  const long long tiles = (M + LM_TILE - 1) / LM_TILE * ((E + LM_TILE - 1) / LM_TILE), pairs = ctx->sm_count / 2;
+  const long long most = (p.words + 4 * LM_KBLOCK - 1) / (4 * LM_KBLOCK);
+  long long split = tiles < pairs ? 2 * pairs / tiles : 1;
+  p.dx_split = (int)(split < most ? split : most);
 
-int prepare_targets(gt_ctx* ctx, const Saved& s, const float* targets, float ignore, const float* ids, const float* teacher, long long M, long long V,
-                    long long K, float T) {
-  GT_CUDA_OK(ctx, cudaMemsetAsync(s.count, 0, sizeof(int), ctx->stream));
-  if (targets) {
-    hard_targets_kernel<<<(unsigned)((M + 255) / 256), 256, 0, ctx->stream>>>(targets, M, V, ignore, s, ctx->d_status);
-  } else {
-    top_targets_kernel<<<(unsigned)((M + 3) / 4), 128, (size_t)4 * 2 * K * 4, ctx->stream>>>(ids, teacher, M, V, (int)K, 1.0f / T, s, ctx->d_status);
+  Carve c = {(char*)saved, 0};
+  l.s = saved_layout(c, M, K);
+  p.x.hi = c.take<uint16_t>(M * p.pitch_e);
+  p.w.hi = c.take<uint16_t>(V * p.pitch_e);
+  if (p.products == 3) { p.x.lo = c.take<uint16_t>(M * p.pitch_e); p.w.lo = c.take<uint16_t>(V * p.pitch_e); }
+  l.saved_bytes = c.at;
+
+  Carve f = {(char*)scratch, 0};                       // the forward pass and the backward pass use it in turn
+  p.counters = f.take<int>(l.pieces + 1);
+  Carve b = f;
+  l.row_loss = f.take<float>(M);
+  p.partial = f.take<float2>((V + LM_TILE - 1) / LM_TILE * 2 * M);
+  for (int i = 0; i < (l.pieces > 1 ? 2 : 1); ++i) {
+    p.g[i].hi = b.take<uint16_t>(M * p.pitch_v);
+    if (p.products == 3) p.g[i].lo = b.take<uint16_t>(M * p.pitch_v);
   }
+  if (p.dx_split > 1) p.dx_partial = b.take<float>(p.dx_split * M * E);
+  l.scratch_bytes = f.at > b.at ? f.at : b.at;
+  p.scalars = l.s.scalars; p.row_of = l.s.row_of; p.stats = l.s.stats; p.factor = l.s.factor; p.ids = l.s.ids; p.q = l.s.q;
+  return l;
+}
+
+int prepare_targets(gt_ctx* ctx, const Saved& s, float* row_loss, const float* targets, float ignore, const float* ids, const float* teacher,
+                    long long M, long long V, long long K, float T) {
+  GT_CUDA_OK(ctx, cudaMemsetAsync(s.scalars, 0, sizeof(LmScalars), ctx->stream));
+  if (targets) {
+    hard_targets_kernel<<<(unsigned)((M + 255) / 256), 256, 0, ctx->stream>>>(targets, M, V, ignore, s, row_loss, ctx->d_status);
+  } else {
+    top_targets_kernel<<<(unsigned)((M + 3) / 4), 128, (size_t)4 * 2 * K * 4, ctx->stream>>>(ids, teacher, M, V, (int)K, 1.0f / T, s, row_loss,
+                                                                                              ctx->d_status);
+  }
+  compact_rows_kernel<<<1, 1024, 0, ctx->stream>>>(M, s);
+  GT_CUDA_OK(ctx, cudaGetLastError());
+  ctx->launches += 2;
+  return GT_OK;
+}
+
+int reduce_loss(gt_ctx* ctx, float* loss, const float* row_loss, long long M, int reduction, const Saved& s) {
+  if (reduction == GT_REDUCE_NONE) return GT_OK;
+  reduce_loss_kernel<<<1, 1024, 0, ctx->stream>>>(loss, row_loss, M, &s.scalars->count, reduction == GT_REDUCE_MEAN);
   GT_CUDA_OK(ctx, cudaGetLastError());
   ctx->launches += 1;
   return GT_OK;
 }
 
-int finish_loss(gt_ctx* ctx, float* loss, float* row_loss, const float* logits, long long ld, const float* x, const float* w, long long M, long long E,
-                long long K, float T, int reduction, const Saved& s) {
-  float* rows = reduction == GT_REDUCE_NONE ? loss : row_loss;
-  row_loss_kernel<<<(unsigned)((M + 7) / 8), 256, 0, ctx->stream>>>(rows, logits, ld, x, w, M, E, (int)K, 1.0f / T, T, s);
-  if (reduction != GT_REDUCE_NONE)
-    reduce_loss_kernel<<<1, 1024, 0, ctx->stream>>>(loss, rows, M, s.count, reduction == GT_REDUCE_MEAN);
-  GT_CUDA_OK(ctx, cudaGetLastError());
-  ctx->launches += reduction == GT_REDUCE_NONE ? 1 : 2;
-  return GT_OK;
-}
-
 int linear_forward(gt_ctx* ctx, float* loss, void* saved, void* scratch, const float* x, const float* w, const float* targets, float ignore,
                    const float* ids, const float* teacher, int64_t M, int64_t V, int64_t E, int64_t K, float T, int reduction, int precision) {
-  const Saved s = saved_layout(saved, M, K);
-  int rc = prepare_targets(ctx, s, targets, ignore, ids, teacher, M, V, K, T);
+  const Linear l = linear_layout(ctx, saved, scratch, M, V, E, K, precision);
+  const Saved& s = l.s;
+  float* rows = reduction == GT_REDUCE_NONE ? loss : l.row_loss;
+  int rc = prepare_targets(ctx, s, rows, targets, ignore, ids, teacher, M, V, K, T);
   if (rc != GT_OK) return rc;
-  float* row_loss = (float*)scratch;
-  float* z = (float*)((char*)scratch + up256(sizeof(float) * M));
-  const long long step = piece_words(M, V), pitch = piece_pitch(step);
-  for (long long v0 = 0; v0 < V; v0 += step) {
-    const long long n = V - v0 < step ? V - v0 : step;
-    rc = gt_gemm(ctx, GT_LAYOUT_NT, M, n, E, x, E, w + v0 * E, E, z, pitch, nullptr, nullptr, 1.0f, 0, GT_EPI_NONE, precision, nullptr);
-    if (rc != GT_OK) return rc;
-    row_stats_kernel<<<(unsigned)M, 256, 0, ctx->stream>>>(z, pitch, n, 1.0f / T, s.stats, v0 > 0);
-    GT_CUDA_OK(ctx, cudaGetLastError());
-    ctx->launches += 1;
-  }
-  return finish_loss(ctx, loss, row_loss, nullptr, 0, x, w, M, E, K, T, reduction, s);
+  GT_CUDA_OK(ctx, cudaMemsetAsync(l.p.counters, 0, sizeof(int), ctx->stream));
+  const long long most = 8ll * ctx->sm_count;
+  auto blocks = [&](long long n) { return (int)((n + 7) / 8 < most ? (n + 7) / 8 : most); };
+  const int bx = blocks(M), bw = blocks(V);
+  largest_kernel<<<(unsigned)(bx + bw), 256, 0, ctx->stream>>>(x, w, V, E, s, bx);
+  split_kernel<<<(unsigned)(bx + bw), 256, 0, ctx->stream>>>(x, w, M, V, E, l.p.pitch_e, s, l.p.x, l.p.w, l.p.products, T, bx);
+  GT_CUDA_OK(ctx, cudaGetLastError());
+  ctx->launches += 2;
+  rc = gt_lm_stats(ctx, l.p);
+  if (rc != GT_OK) return rc;
+  linear_row_loss_kernel<<<(unsigned)((M + 7) / 8), 256, 0, ctx->stream>>>(rows, l.p.partial, (int)((V + LM_TILE - 1) / LM_TILE * 2), x, w, M, E, (int)K, T, s);
+  GT_CUDA_OK(ctx, cudaGetLastError());
+  ctx->launches += 1;
+  return reduce_loss(ctx, loss, rows, M, reduction, s);
 }
 
 }  // namespace
 
 extern "C" int gt_linear_loss_sizes(gt_ctx* ctx, int64_t M, int64_t V, int64_t E, int64_t K, int precision, size_t* saved, size_t* scratch) {
-  if (!ctx || !saved || !scratch || E <= 0 || bad_sizes(M, V, K) || bad_precision(precision)) return GT_ERR_INVALID_ARG;
-  *saved = saved_layout(nullptr, M, K).bytes;
-  *scratch = up256(sizeof(float) * M) + sizeof(float) * M * piece_pitch(piece_words(M, V));
+  if (!ctx || !saved || !scratch || bad_sizes(M, V, K) || bad_width(E) || bad_precision(precision)) return GT_ERR_INVALID_ARG;
+  const Linear l = linear_layout(ctx, nullptr, nullptr, M, V, E, K, precision);
+  *saved = l.saved_bytes;
+  *scratch = l.scratch_bytes;
   return GT_OK;
 }
 
 extern "C" int gt_linear_cross_entropy(gt_ctx* ctx, float* loss, void* saved, void* scratch, const float* x, const float* w, const float* targets,
                                        int64_t M, int64_t V, int64_t E, float ignore_index, int reduction, int precision) {
-  if (!ctx || !loss || !saved || !scratch || !x || !w || !targets || E <= 0 || bad_sizes(M, V, 1) || bad_reduction(reduction) || bad_precision(precision)) return GT_ERR_INVALID_ARG;
+  if (!ctx || !loss || !saved || !scratch || !x || !w || !targets || bad_sizes(M, V, 1) || bad_width(E) || bad_reduction(reduction) ||
+      bad_precision(precision)) return GT_ERR_INVALID_ARG;
   return linear_forward(ctx, loss, saved, scratch, x, w, targets, ignore_index, nullptr, nullptr, M, V, E, 1, 1.0f, reduction, precision);
 }
 
 extern "C" int gt_linear_topk_distillation(gt_ctx* ctx, float* loss, void* saved, void* scratch, const float* x, const float* w, const float* ids,
                                            const float* teacher, int64_t M, int64_t V, int64_t E, int64_t K, float temperature, int reduction,
                                            int precision) {
-  if (!ctx || !loss || !saved || !scratch || !x || !w || !ids || !teacher || E <= 0 || bad_sizes(M, V, K) || bad_reduction(reduction) ||
+  if (!ctx || !loss || !saved || !scratch || !x || !w || !ids || !teacher || bad_sizes(M, V, K) || bad_width(E) || bad_reduction(reduction) ||
       bad_temperature(temperature) || bad_precision(precision)) return GT_ERR_INVALID_ARG;
   return linear_forward(ctx, loss, saved, scratch, x, w, nullptr, 0.0f, ids, teacher, M, V, E, K, temperature, reduction, precision);
 }
@@ -349,25 +597,28 @@ extern "C" int gt_linear_topk_distillation(gt_ctx* ctx, float* loss, void* saved
 extern "C" int gt_linear_loss_backward(gt_ctx* ctx, float* dx, float* dw, void* saved, void* scratch, const float* x, const float* w,
                                        const float* upstream, int64_t M, int64_t V, int64_t E, int64_t K, float temperature, int reduction,
                                        int precision, int acc_dx, int acc_dw) {
-  if (!ctx || !saved || !scratch || !x || !w || !upstream || E <= 0 || bad_sizes(M, V, K) || bad_reduction(reduction) || bad_temperature(temperature) ||
-      bad_precision(precision)) return GT_ERR_INVALID_ARG;
-  const Saved s = saved_layout(saved, M, K);
-  float* z = (float*)((char*)scratch + up256(sizeof(float) * M));
-  const long long step = piece_words(M, V), pitch = piece_pitch(step);
-  for (long long v0 = 0; v0 < V; v0 += step) {
-    const long long n = V - v0 < step ? V - v0 : step;
-    int rc = gt_gemm(ctx, GT_LAYOUT_NT, M, n, E, x, E, w + v0 * E, E, z, pitch, nullptr, nullptr, 1.0f, 0, GT_EPI_NONE, precision, nullptr);
-    if (rc != GT_OK) return rc;
-    row_grad_kernel<<<(unsigned)M, 256, 0, ctx->stream>>>(z, pitch, z, pitch, v0, n, 1.0f / temperature, temperature, s, (int)K, upstream, reduction, 0);
+  if (!ctx || !saved || !scratch || !x || !w || !upstream || bad_sizes(M, V, K) || bad_width(E) || bad_reduction(reduction) ||
+      bad_temperature(temperature) || bad_precision(precision)) return GT_ERR_INVALID_ARG;
+  if (!dx && !dw) return GT_OK;
+  Linear l = linear_layout(ctx, saved, scratch, M, V, E, K, precision);
+  LmProblem& p = l.p;
+  p.dx = dx; p.dw = dw; p.acc_dx = acc_dx; p.acc_dw = acc_dw;
+  GT_CUDA_OK(ctx, cudaMemsetAsync(p.counters, 0, sizeof(int) * (l.pieces + 1), ctx->stream));
+  grad_factor_kernel<<<1, 1024, 0, ctx->stream>>>(upstream, reduction, temperature, l.s);
+  GT_CUDA_OK(ctx, cudaGetLastError());
+  ctx->launches += 1;
+  if (dx && !acc_dx) {
+    zero_rows_kernel<<<(unsigned)M, 128, 0, ctx->stream>>>(dx, E, l.s);
     GT_CUDA_OK(ctx, cudaGetLastError());
     ctx->launches += 1;
-    if (dx) {
-      rc = gt_gemm(ctx, GT_LAYOUT_NN, M, E, n, z, pitch, w + v0 * E, E, dx, E, nullptr, nullptr, 1.0f, acc_dx || v0 > 0, GT_EPI_NONE, precision, nullptr);
-      if (rc != GT_OK) return rc;
-    }
-    if (dw) {
-      rc = gt_gemm(ctx, GT_LAYOUT_TN, n, E, M, z, pitch, x, E, dw + v0 * E, E, nullptr, nullptr, 1.0f, acc_dw, GT_EPI_NONE, precision, nullptr);
-      if (rc != GT_OK) return rc;
+  }
+  for (int piece = 0; piece <= l.pieces; ++piece) {
+    int rc = gt_lm_step(ctx, p, piece);
+    if (rc != GT_OK) return rc;
+    if (piece > 0 && dx && p.dx_split > 1) {
+      add_shares_kernel<<<(unsigned)M, 256, 0, ctx->stream>>>(dx, p.dx_partial, p.dx_split, M, E, acc_dx || piece > 1, l.s);
+      GT_CUDA_OK(ctx, cudaGetLastError());
+      ctx->launches += 1;
     }
   }
   return GT_OK;
@@ -384,12 +635,14 @@ extern "C" int gt_topk_distillation(gt_ctx* ctx, float* loss, void* saved, const
   if (!ctx || !loss || !saved || !logits || !ids || !teacher || bad_sizes(B, C, K) || ld_logits < C || bad_reduction(reduction) ||
       bad_temperature(temperature)) return GT_ERR_INVALID_ARG;
   const Saved s = saved_layout(saved, B, K);
-  int rc = prepare_targets(ctx, s, nullptr, 0.0f, ids, teacher, B, C, K, temperature);
+  float* rows = reduction == GT_REDUCE_NONE ? loss : (float*)((char*)saved + s.bytes);
+  int rc = prepare_targets(ctx, s, rows, nullptr, 0.0f, ids, teacher, B, C, K, temperature);
   if (rc != GT_OK) return rc;
-  row_stats_kernel<<<(unsigned)B, 256, 0, ctx->stream>>>(logits, ld_logits, C, 1.0f / temperature, s.stats, 0);
+  row_stats_kernel<<<(unsigned)B, 256, 0, ctx->stream>>>(logits, ld_logits, C, 1.0f / temperature, s.stats);
+  row_loss_kernel<<<(unsigned)((B + 7) / 8), 256, 0, ctx->stream>>>(rows, logits, ld_logits, B, (int)K, 1.0f / temperature, temperature, s);
   GT_CUDA_OK(ctx, cudaGetLastError());
-  ctx->launches += 1;
-  return finish_loss(ctx, loss, (float*)((char*)saved + s.bytes), logits, ld_logits, nullptr, nullptr, B, 0, K, temperature, reduction, s);
+  ctx->launches += 2;
+  return reduce_loss(ctx, loss, rows, B, reduction, s);
 }
 
 extern "C" int gt_topk_distillation_backward(gt_ctx* ctx, float* dlogits, int64_t ld_dlogits, void* saved, const float* logits, int64_t ld_logits,
@@ -398,7 +651,7 @@ extern "C" int gt_topk_distillation_backward(gt_ctx* ctx, float* dlogits, int64_
   if (!ctx || !dlogits || !saved || !logits || !upstream || bad_sizes(B, C, K) || ld_logits < C || ld_dlogits < C || bad_reduction(reduction) ||
       bad_temperature(temperature)) return GT_ERR_INVALID_ARG;
   const Saved s = saved_layout(saved, B, K);
-  row_grad_kernel<<<(unsigned)B, 256, 0, ctx->stream>>>(dlogits, ld_dlogits, logits, ld_logits, 0, C, 1.0f / temperature, temperature, s, (int)K,
+  row_grad_kernel<<<(unsigned)B, 256, 0, ctx->stream>>>(dlogits, ld_dlogits, logits, ld_logits, C, 1.0f / temperature, temperature, s, (int)K,
                                                         upstream, reduction, accumulate);
   GT_CUDA_OK(ctx, cudaGetLastError());
   ctx->launches += 1;
