@@ -7,7 +7,7 @@
 // by fp16 tensor-core instructions, which run at twice the rate of tf32 and read half the bytes.  With products == 1 only hi hi'
 // is taken: the operand rounding of tf32.
 // The tensor cores add into their 32-bit accumulators by cutting off, not rounding (measured: a sum of K = 512 terms of one
-// sign comes out 1.5e-6 too small).  So no accumulator stays there for long: after SUB_K of K (two stages, 24 additions) the
+// sign comes out 1.5e-6 too small).  So no accumulator stays there for long: after three stages (192 of K) the
 // epilogue warps add it to their registers, rounding to nearest, while the next one fills the other half of tensor memory.
 //
 // Work.  One kernel, persistent, a pair of CTAs (cta_group::2) per 256 x 256 tile, handed out by a counter: the units of a launch
@@ -218,7 +218,10 @@ __global__ void __launch_bounds__(THREADS, 1) lm_pair_kernel(const __grid_consta
           if (++slot == SLOTS) { slot = 0; slot_ph ^= 1u; }
         } else if (!take_unit(false, u)) { ok = false; break; }
         if (!unit_of(p, rows, u, t)) break;
-        if (rank == 0) next = atomicAdd(p.counter, 1);          // back by the time this unit's loads have been issued
+        // The next unit is asked for near this one's end: its number is back in time, and a pair in a long unit does not sit on
+        // work that others could do (asked for at the start, a pass over 8192 x 768 x 50257 took 7.95 ms instead of 6.91).
+        const int ask = max(t.kb_lo, t.kb_hi - 2);
+        if (rank == 0 && t.kb_lo >= t.kb_hi) next = atomicAdd(p.counter, 1);
         const CUtensorMap* ma = t.kind == DX || t.kind == DW ? maps.g_mul : maps.x;
         const CUtensorMap* mb = t.kind == DW ? maps.x : maps.w;
         const bool a_mn = t.kind == DW, b_mn = t.kind == DX || t.kind == DW;
@@ -229,7 +232,10 @@ __global__ void __launch_bounds__(THREADS, 1) lm_pair_kernel(const __grid_consta
         if (t.kind == DX) bk = p.v0_mul;
         for (int kb = t.kb_lo; kb < t.kb_hi; ++kb) {
           if (!mbar_wait_cluster(bar_empty + 8 * s, ph ^ 1u, abort_flag, p.status)) { ok = false; break; }
-          if (rank == 0) mbar_expect_tx(bar_full + 8 * s, 2 * stage_bytes);
+          if (rank == 0) {
+            mbar_expect_tx(bar_full + 8 * s, 2 * stage_bytes);
+            if (kb == ask) next = atomicAdd(p.counter, 1);
+          }
           const uint32_t full = leader_full + 8 * s;
           const uint32_t st = ring + s * stage_bytes;
           const int k0 = kb * BK;
@@ -544,9 +550,11 @@ Params common_params(gt_ctx* ctx, const LmProblem& p) {
   a.partial = p.partial;
   a.E = p.E; a.M = (int)p.M; a.V = (int)p.V;
   a.products = p.products;
-  // Between two roundings to nearest: 128 of K with three products (24 additions), 512 with one, whose operands are
-  // rounded to 11 bits anyway.
-  a.sub_stages = p.products == 3 ? 2 : 8;
+  // Between two roundings to nearest: 192 of K with three products (36 additions), 512 with one, whose operands are rounded to 11
+  // bits anyway.  Every hand-over costs the tensor cores about 450 cycles.  8192 x 768 x 50257 with gradients, by stages of 64
+  // between two hand-overs, time and error of dx against 64 bits: 2: 6.91 ms, 3.0e-7; 3: 6.46 ms, 4.3e-7; 4: 6.46 ms,
+  // 5.8e-7; 6: 6.31 ms, 8.6e-7.
+  a.sub_stages = p.products == 3 ? 3 : 8;
   a.dx_split = 1;
   return a;
 }
