@@ -145,8 +145,8 @@ SIGNATURES = {
     "gt_linear_topk_distillation": (c_int, [c_void_p] + [c_void_p] * 7 + [c_int64] * 4 + [c_float, c_int, c_int]),
     "gt_linear_loss_backward": (c_int, [c_void_p] + [c_void_p] * 7 + [c_int64] * 4 + [c_float, c_int, c_int, c_int, c_int]),
     "gt_topk_distillation_sizes": (c_int, [c_void_p, c_int64, c_int64, c_int64, POINTER(c_size_t)]),
-    "gt_topk_distillation": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64,
-                                     c_float, c_int]),
+    "gt_topk_distillation": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64,
+                                     c_int64, c_int64, c_float, c_int]),
     "gt_topk_distillation_backward": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64,
                                               c_float, c_int, c_int]),
     "gt_adamw": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_float, c_float, c_float, c_float,

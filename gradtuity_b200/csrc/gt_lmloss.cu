@@ -1,4 +1,5 @@
-// Losses of the language-model head with sparse targets, and their gradients.
+// Losses of the language-model head with sparse targets, and their gradients: the targets, and the linear forms.
+// (Distillation of given logits: gt_distill.cu.)
 //
 // For token t and word v, z_tv = logit_tv / T (T = 1 for cross entropy; the linear forms compute logit = x W^T themselves):
 //     p_tv = exp(z_tv - m_t) / s_t,  m_t = max_v z_tv,  s_t = sum_v exp(z_tv - m_t)
@@ -21,8 +22,6 @@
 
 namespace {
 
-constexpr int TOP_MAX = 1024;                       // targets of a row: they are sorted in shared memory
-constexpr int UNUSED = 0x7fffffff;                  // id of a place that is not in use; sorts behind every word
 constexpr long long PIECE_BYTES = 64ll << 20;       // what G of one piece of the vocabulary may occupy
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -36,66 +35,11 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
-// (maximum, sum of exponentials relative to it); an empty part is (-inf, 0).  A maximum of -inf on both sides stays (-inf, 0):
-// every exponential is then 0, which the caller sees as a sum of 0.
-struct MaxSum { float m, s; };
-__device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b) {
-  const float m = fmaxf(a.m, b.m);
-  if (m == -INFINITY) return {m, a.s + b.s};
-  return {m, a.s * expf(a.m - m) + b.s * expf(b.m - m)};
-}
-__device__ __forceinline__ MaxSum warp_join(MaxSum a) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    MaxSum b;
-    b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
-    b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
-    // the same order of the two operands on both lanes, so that all lanes hold the same bits
-    a = (threadIdx.x & o) ? join(b, a) : join(a, b);
-  }
-  return a;
-}
-
-// What the forward pass leaves for the backward pass, in one block of memory.
-struct Saved {
-  LmScalars* scalars;
-  float* weight;    // by row: 1, or 0 for a row that does not count
-  float* konst;     // by row: sum of q log q
-  int* ids;         // (M, K), ascending, UNUSED at the end
-  float* q;         // (M, K), 0 where unused
-  int* row_of;      // rows that count, in order
-  float2* stats;    // by row (distillation of given logits), or by compact row and with m in units of log 2 (linear forms)
-  float2* factor;   // by compact row, see LmProblem
-  size_t bytes;
-};
-size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
-struct Carve {
-  char* p; size_t at;
-  template <class T> T* take(size_t n) { T* r = (T*)(p + at); at += up256(n * sizeof(T)); return r; }
-};
-Saved saved_layout(Carve& c, long long M, long long K) {
-  Saved s;
-  s.scalars = c.take<LmScalars>(1);
-  s.weight = c.take<float>(M);
-  s.konst = c.take<float>(M);
-  s.ids = c.take<int>(M * K);
-  s.q = c.take<float>(M * K);
-  s.row_of = c.take<int>(M);
-  s.stats = c.take<float2>(M);
-  s.factor = c.take<float2>(M);
-  s.bytes = c.at;
-  return s;
-}
-Saved saved_layout(void* base, long long M, long long K) {
-  Carve c = {(char*)base, 0};
-  return saved_layout(c, M, K);
-}
-
 // ---- targets -------------------------------------------------------------------------------------
 
 // Cross entropy: one target of q = 1 per row.  An id outside the vocabulary sets the status word.
 __global__ void __launch_bounds__(256) hard_targets_kernel(const float* __restrict__ targets, long long M, long long V, float ignore,
-                                                           Saved s, float* __restrict__ row_loss, int* status) {
+                                                           LmSaved s, float* __restrict__ row_loss, int* status) {
   const long long t = (long long)blockIdx.x * blockDim.x + threadIdx.x;
   bool used = false;
   if (t < M) {
@@ -103,7 +47,7 @@ __global__ void __launch_bounds__(256) hard_targets_kernel(const float* __restri
     const bool in_range = f >= 0.0f && f < (float)V;
     used = f != ignore && in_range;
     if (f != ignore && !in_range) atomicExch(status, GT_ERR_INVALID_ARG);
-    s.ids[t] = used ? (int)f : UNUSED;
+    s.ids[t] = used ? (int)f : LM_UNUSED;
     s.q[t] = used ? 1.0f : 0.0f;
     s.weight[t] = used ? 1.0f : 0.0f;
     s.konst[t] = 0.0f;
@@ -114,7 +58,7 @@ __global__ void __launch_bounds__(256) hard_targets_kernel(const float* __restri
 // Distillation: a warp per row.  q = softmax(teacher / T) over the places in use (id >= 0, logit above -inf), sorted by id by
 // counting, for each place, the places that go before it (K^2 comparisons, K is tens to a few hundred).
 __global__ void __launch_bounds__(128) top_targets_kernel(const float* __restrict__ ids, const float* __restrict__ teacher, long long M,
-                                                          long long V, int K, float inv_T, Saved s,
+                                                          long long V, int K, float inv_T, LmSaved s,
                                                           float* __restrict__ row_loss, int* status) {
   extern __shared__ float smem[];
   const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
@@ -129,7 +73,7 @@ __global__ void __launch_bounds__(128) top_targets_kernel(const float* __restric
       const float f = ids[t * K + k], v = teacher[t * K + k];
       bool used = !(f < 0.0f) && v > -INFINITY;
       if (used && !(f < (float)V)) { atomicExch(status, GT_ERR_INVALID_ARG); used = false; }
-      key[k] = used ? (int)f : UNUSED;
+      key[k] = used ? (int)f : LM_UNUSED;
       val[k] = used ? v : -INFINITY;
       if (used) { any = true; mx = fmaxf(mx, v); }
     }
@@ -138,7 +82,7 @@ __global__ void __launch_bounds__(128) top_targets_kernel(const float* __restric
     __syncwarp();
     float sum = 0.0f;
     for (int k = l; k < K; k += 32)
-      if (key[k] != UNUSED) sum += expf((val[k] - mx) * inv_T);
+      if (key[k] != LM_UNUSED) sum += expf((val[k] - mx) * inv_T);
     sum = warp_sum(sum);
     const float log_sum = logf(sum), inv = 1.0f / sum;
     float konst = 0.0f;
@@ -150,7 +94,7 @@ __global__ void __launch_bounds__(128) top_targets_kernel(const float* __restric
         before += (o < id) || (o == id && j < k);
       }
       float q = 0.0f;
-      if (id != UNUSED) {
+      if (id != LM_UNUSED) {
         const float u = (val[k] - mx) * inv_T;
         q = expf(u) * inv;
         if (q != 0.0f) konst += q * (u - log_sum);          // 0 log 0 = 0
@@ -162,13 +106,14 @@ __global__ void __launch_bounds__(128) top_targets_kernel(const float* __restric
     if (l == 0) {
       s.weight[t] = any ? 1.0f : 0.0f;
       s.konst[t] = konst;
-      if (!any) row_loss[t] = 0.0f;
+      if (any) atomicAdd(&s.scalars->count, 1);             // whole numbers: the order does not matter
+      else row_loss[t] = 0.0f;
     }
   }
 }
 
 // row_of: the rows that count, in order; count: how many.  One block.
-__global__ void __launch_bounds__(1024) compact_rows_kernel(long long M, Saved s) {
+__global__ void __launch_bounds__(1024) compact_rows_kernel(long long M, LmSaved s) {
   __shared__ int sums[32];
   const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
   int base = 0;
@@ -195,7 +140,7 @@ __global__ void __launch_bounds__(1024) compact_rows_kernel(long long M, Saved s
 // ---- operands of the linear forms: largest value, then the split into halves ------------------------
 
 // Whole matrix w, and of x the rows that count.  A maximum of bits as whole numbers, so the order of the additions is no matter.
-__global__ void __launch_bounds__(256) largest_kernel(const float* __restrict__ x, const float* __restrict__ w, long long V, long long E, Saved s,
+__global__ void __launch_bounds__(256) largest_kernel(const float* __restrict__ x, const float* __restrict__ w, long long V, long long E, LmSaved s,
                                                       int blocks_x) {
   const bool is_x = (int)blockIdx.x < blocks_x;
   const long long rows = is_x ? s.scalars->count : V;
@@ -238,7 +183,7 @@ __device__ __forceinline__ int scale_exponent(unsigned amax) {
 
 // A warp per row.  x: compact rows, and zeros behind them to the end of the last tile of rows.
 __global__ void __launch_bounds__(256) split_kernel(const float* __restrict__ x, const float* __restrict__ w, long long M, long long V, long long E,
-                                                    long long pitch, Saved s, LmSplit xs, LmSplit ws, int products, float T, int blocks_x) {
+                                                    long long pitch, LmSaved s, LmSplit xs, LmSplit ws, int products, float T, int blocks_x) {
   const int l = threadIdx.x & 31;
   const bool is_x = (int)blockIdx.x < blocks_x;
   const int ex = scale_exponent(s.scalars->amax_x), ew = scale_exponent(s.scalars->amax_w);
@@ -285,86 +230,11 @@ __global__ void __launch_bounds__(256) split_kernel(const float* __restrict__ x,
 
 // ---- rows ------------------------------------------------------------------------------------------
 
-// (m, s) of a row of `n` values scaled by `scale`.  A block per row.
-__global__ void __launch_bounds__(256) row_stats_kernel(const float* __restrict__ z, long long ld, long long n, float scale,
-                                                        float2* __restrict__ stats) {
-  __shared__ MaxSum part[8];
-  const long long t = blockIdx.x;
-  const float* zr = z + t * ld;
-  MaxSum a = {-INFINITY, 0.0f};
-  for (long long j = threadIdx.x; j < n; j += blockDim.x) {
-    const float v = zr[j] * scale;
-    if (v > a.m) { a.s = a.s * expf(a.m - v) + 1.0f; a.m = v; }
-    else if (v != -INFINITY) { a.s += expf(v - a.m); }
-  }
-  a = warp_join(a);
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = a;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    MaxSum r = {-INFINITY, 0.0f};
-    for (int w = 0; w < 8; ++w) r = join(r, part[w]);
-    stats[t] = make_float2(r.m, r.s);
-  }
-}
-
-// The gradient of the loss with respect to given logits: g = c (p - q), where c holds the row's weight, T, the upstream gradient
-// and 1 / n.  A block per row.
-__global__ void __launch_bounds__(256) row_grad_kernel(float* __restrict__ g, long long ld_g, const float* z, long long ld, long long n, float scale,
-                                                       float T, Saved s, int K, const float* __restrict__ upstream, int reduction, int accumulate) {
-  const long long t = blockIdx.x;
-  const float* zr = z + t * ld;
-  float* gr = g + t * ld_g;
-  float c = s.weight[t] * T;
-  if (c != 0.0f) {
-    c *= reduction == GT_REDUCE_NONE ? upstream[t] : upstream[0];
-    if (reduction == GT_REDUCE_MEAN) c /= (float)s.scalars->count;
-  }
-  if (s.weight[t] == 0.0f) {
-    if (!accumulate) for (long long j = threadIdx.x; j < n; j += blockDim.x) gr[j] = 0.0f;
-    return;
-  }
-  const float2 st = s.stats[t];
-  const float m = st.x, cs = c / st.y;
-  for (long long j = threadIdx.x; j < n; j += blockDim.x) {
-    const float v = cs * expf(zr[j] * scale - m);
-    gr[j] = accumulate ? gr[j] + v : v;
-  }
-  __syncthreads();
-  const int* ids = s.ids + t * K;
-  const float* q = s.q + t * K;
-  for (int k = threadIdx.x; k < K; k += blockDim.x) {
-    const int id = ids[k];
-    if (id == UNUSED || (k > 0 && ids[k - 1] == id)) continue;     // the first of a run of equal ids takes them all
-    float sum = 0.0f;
-    for (int j = k; j < K && ids[j] == id; ++j) sum += q[j];
-    gr[id] -= c * sum;
-  }
-}
-
-// loss_t of given logits from the row's statistics: a warp per row.
-__global__ void __launch_bounds__(256) row_loss_kernel(float* __restrict__ row_loss, const float* __restrict__ logits, long long ld, long long M, int K,
-                                                       float scale, float T, Saved s) {
-  const long long t = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int l = threadIdx.x & 31;
-  if (t >= M || s.weight[t] == 0.0f) return;
-  const float2 st = s.stats[t];
-  const float log_s = logf(st.y);
-  float cross = 0.0f;
-  for (int k = l; k < K; k += 32) {
-    const int id = s.ids[t * K + k];
-    if (id == UNUSED) break;
-    const float q = s.q[t * K + k];
-    if (q != 0.0f) cross += q * ((logits[t * ld + id] * scale - st.x) - log_s);
-  }
-  cross = warp_sum(cross);
-  if (l == 0) row_loss[t] = T * T * (s.konst[t] - cross);
-}
-
 // The linear forms: joins the tiles' maxima and sums of a compact row, takes the logits of its targets in 32 bits straight from
 // x and w, and writes the row's loss.  A warp per row.
 __global__ void __launch_bounds__(256) linear_row_loss_kernel(float* __restrict__ row_loss, const float2* __restrict__ partial, int parts,
                                                               const float* __restrict__ x, const float* __restrict__ w, long long M, long long E,
-                                                              int K, float T, Saved s) {
+                                                              int K, float T, LmSaved s) {
   const long long i = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int l = threadIdx.x & 31;
   if (i >= s.scalars->count) return;
@@ -383,7 +253,7 @@ __global__ void __launch_bounds__(256) linear_row_loss_kernel(float* __restrict_
   float cross = 0.0f;
   for (int k = 0; k < K; ++k) {
     const int id = s.ids[t * K + k];
-    if (id == UNUSED) break;
+    if (id == LM_UNUSED) break;
     const float q = s.q[t * K + k];
     if (q == 0.0f) continue;
     float z = 0.0f;
@@ -399,7 +269,7 @@ __global__ void __launch_bounds__(256) linear_row_loss_kernel(float* __restrict_
 
 // What the rows' gradients are multiplied by.  The halves of G hold 2^14 u (p - q), u = 1, or with a gradient per row that row's
 // share of a power of two P above the largest; the rest goes into the products' own factors.  One block.
-__global__ void __launch_bounds__(1024) grad_factor_kernel(const float* __restrict__ upstream, int reduction, float T, Saved s) {
+__global__ void __launch_bounds__(1024) grad_factor_kernel(const float* __restrict__ upstream, int reduction, float T, LmSaved s) {
   __shared__ unsigned part[32];
   const int n = s.scalars->count;
   float P = 1.0f;
@@ -429,7 +299,7 @@ __global__ void __launch_bounds__(1024) grad_factor_kernel(const float* __restri
 }
 
 // dx of rows that do not count.  A block per row.
-__global__ void __launch_bounds__(128) zero_rows_kernel(float* __restrict__ dx, long long E, Saved s) {
+__global__ void __launch_bounds__(128) zero_rows_kernel(float* __restrict__ dx, long long E, LmSaved s) {
   const long long t = blockIdx.x;
   if (s.weight[t] != 0.0f) return;
   for (long long e = threadIdx.x; e < E; e += 128) dx[t * E + e] = 0.0f;
@@ -437,7 +307,7 @@ __global__ void __launch_bounds__(128) zero_rows_kernel(float* __restrict__ dx, 
 
 // dx (+)= the shares of a piece, in order.
 __global__ void __launch_bounds__(256) add_shares_kernel(float* __restrict__ dx, const float* __restrict__ shares, int n_shares, long long M, long long E,
-                                                         int add, Saved s) {
+                                                         int add, LmSaved s) {
   const long long i = blockIdx.x;
   if (i >= s.scalars->count) return;
   float* to = dx + (long long)s.row_of[i] * E;
@@ -465,18 +335,13 @@ __global__ void __launch_bounds__(1024) reduce_loss_kernel(float* __restrict__ l
   }
 }
 
-bool bad_sizes(long long M, long long V, long long K) {
-  return M <= 0 || V <= 0 || K <= 0 || M > 0x7fffffff || V >= (1ll << 24) || K > TOP_MAX;    // ids are float-encoded: exact below 2^24
-}
 bool bad_width(long long E) { return E <= 0 || E > (1 << 24); }
-bool bad_temperature(float T) { return !(T > 0.0f) || isinf(T); }
-bool bad_reduction(int r) { return r != GT_REDUCE_NONE && r != GT_REDUCE_MEAN && r != GT_REDUCE_SUM; }
 
 bool bad_precision(int p) { return p != GT_PREC_TF32 && p != GT_PREC_TF32X3 && p != GT_PREC_FP32; }
 
 // How a linear form's work is cut up, and where everything lies.
 struct Linear {
-  Saved s;
+  LmSaved s;
   LmProblem p;
   float* row_loss;
   int pieces;
@@ -501,16 +366,16 @@ Linear linear_layout(gt_ctx* ctx, void* saved, void* scratch, long long M, long 
   long long split = tiles < pairs ? 2 * pairs / tiles : 1;
   p.dx_split = (int)(split < most ? split : most);
 
-  Carve c = {(char*)saved, 0};
-  l.s = saved_layout(c, M, K);
+  LmCarve c = {(char*)saved, 0};
+  l.s = lm_saved(c, M, K);
   p.x.hi = c.take<uint16_t>(M * p.pitch_e);
   p.w.hi = c.take<uint16_t>(V * p.pitch_e);
   if (p.products == 3) { p.x.lo = c.take<uint16_t>(M * p.pitch_e); p.w.lo = c.take<uint16_t>(V * p.pitch_e); }
   l.saved_bytes = c.at;
 
-  Carve f = {(char*)scratch, 0};                       // the forward pass and the backward pass use it in turn
+  LmCarve f = {(char*)scratch, 0};                       // the forward pass and the backward pass use it in turn
   p.counters = f.take<int>(l.pieces + 1);
-  Carve b = f;
+  LmCarve b = f;
   l.row_loss = f.take<float>(M);
   p.partial = f.take<float2>((V + LM_TILE - 1) / LM_TILE * 2 * M);
   for (int i = 0; i < (l.pieces > 1 ? 2 : 1); ++i) {
@@ -523,22 +388,23 @@ Linear linear_layout(gt_ctx* ctx, void* saved, void* scratch, long long M, long 
   return l;
 }
 
-int prepare_targets(gt_ctx* ctx, const Saved& s, float* row_loss, const float* targets, float ignore, const float* ids, const float* teacher,
+int prepare_linear(gt_ctx* ctx, const LmSaved& s, float* row_loss, const float* targets, float ignore, const float* ids, const float* teacher,
                     long long M, long long V, long long K, float T) {
-  GT_CUDA_OK(ctx, cudaMemsetAsync(s.scalars, 0, sizeof(LmScalars), ctx->stream));
   if (targets) {
+    GT_CUDA_OK(ctx, cudaMemsetAsync(s.scalars, 0, sizeof(LmScalars), ctx->stream));
     hard_targets_kernel<<<(unsigned)((M + 255) / 256), 256, 0, ctx->stream>>>(targets, M, V, ignore, s, row_loss, ctx->d_status);
+    ctx->launches += 1;
   } else {
-    top_targets_kernel<<<(unsigned)((M + 3) / 4), 128, (size_t)4 * 2 * K * 4, ctx->stream>>>(ids, teacher, M, V, (int)K, 1.0f / T, s, row_loss,
-                                                                                              ctx->d_status);
+    int rc = gt_lm_top_targets(ctx, s, row_loss, ids, teacher, M, V, K, T);
+    if (rc != GT_OK) return rc;
   }
   compact_rows_kernel<<<1, 1024, 0, ctx->stream>>>(M, s);
   GT_CUDA_OK(ctx, cudaGetLastError());
-  ctx->launches += 2;
+  ctx->launches += 1;
   return GT_OK;
 }
 
-int reduce_loss(gt_ctx* ctx, float* loss, const float* row_loss, long long M, int reduction, const Saved& s) {
+int reduce_loss(gt_ctx* ctx, float* loss, const float* row_loss, long long M, int reduction, const LmSaved& s) {
   if (reduction == GT_REDUCE_NONE) return GT_OK;
   reduce_loss_kernel<<<1, 1024, 0, ctx->stream>>>(loss, row_loss, M, &s.scalars->count, reduction == GT_REDUCE_MEAN);
   GT_CUDA_OK(ctx, cudaGetLastError());
@@ -549,9 +415,9 @@ int reduce_loss(gt_ctx* ctx, float* loss, const float* row_loss, long long M, in
 int linear_forward(gt_ctx* ctx, float* loss, void* saved, void* scratch, const float* x, const float* w, const float* targets, float ignore,
                    const float* ids, const float* teacher, int64_t M, int64_t V, int64_t E, int64_t K, float T, int reduction, int precision) {
   const Linear l = linear_layout(ctx, saved, scratch, M, V, E, K, precision);
-  const Saved& s = l.s;
+  const LmSaved& s = l.s;
   float* rows = reduction == GT_REDUCE_NONE ? loss : l.row_loss;
-  int rc = prepare_targets(ctx, s, rows, targets, ignore, ids, teacher, M, V, K, T);
+  int rc = prepare_linear(ctx, s, rows, targets, ignore, ids, teacher, M, V, K, T);
   if (rc != GT_OK) return rc;
   GT_CUDA_OK(ctx, cudaMemsetAsync(l.p.counters, 0, sizeof(int), ctx->stream));
   const long long most = 8ll * ctx->sm_count;
@@ -571,8 +437,17 @@ int linear_forward(gt_ctx* ctx, float* loss, void* saved, void* scratch, const f
 
 }  // namespace
 
+int gt_lm_top_targets(gt_ctx* ctx, const LmSaved& s, float* row_loss, const float* ids, const float* teacher, long long M, long long V, long long K,
+                      float T) {
+  GT_CUDA_OK(ctx, cudaMemsetAsync(s.scalars, 0, sizeof(LmScalars), ctx->stream));
+  top_targets_kernel<<<(unsigned)((M + 3) / 4), 128, (size_t)4 * 2 * K * 4, ctx->stream>>>(ids, teacher, M, V, (int)K, 1.0f / T, s, row_loss, ctx->d_status);
+  GT_CUDA_OK(ctx, cudaGetLastError());
+  ctx->launches += 1;
+  return GT_OK;
+}
+
 extern "C" int gt_linear_loss_sizes(gt_ctx* ctx, int64_t M, int64_t V, int64_t E, int64_t K, int precision, size_t* saved, size_t* scratch) {
-  if (!ctx || !saved || !scratch || bad_sizes(M, V, K) || bad_width(E) || bad_precision(precision)) return GT_ERR_INVALID_ARG;
+  if (!ctx || !saved || !scratch || lm_bad_sizes(M, V, K) || bad_width(E) || bad_precision(precision)) return GT_ERR_INVALID_ARG;
   const Linear l = linear_layout(ctx, nullptr, nullptr, M, V, E, K, precision);
   *saved = l.saved_bytes;
   *scratch = l.scratch_bytes;
@@ -581,7 +456,7 @@ extern "C" int gt_linear_loss_sizes(gt_ctx* ctx, int64_t M, int64_t V, int64_t E
 
 extern "C" int gt_linear_cross_entropy(gt_ctx* ctx, float* loss, void* saved, void* scratch, const float* x, const float* w, const float* targets,
                                        int64_t M, int64_t V, int64_t E, float ignore_index, int reduction, int precision) {
-  if (!ctx || !loss || !saved || !scratch || !x || !w || !targets || bad_sizes(M, V, 1) || bad_width(E) || bad_reduction(reduction) ||
+  if (!ctx || !loss || !saved || !scratch || !x || !w || !targets || lm_bad_sizes(M, V, 1) || bad_width(E) || lm_bad_reduction(reduction) ||
       bad_precision(precision)) return GT_ERR_INVALID_ARG;
   return linear_forward(ctx, loss, saved, scratch, x, w, targets, ignore_index, nullptr, nullptr, M, V, E, 1, 1.0f, reduction, precision);
 }
@@ -589,16 +464,16 @@ extern "C" int gt_linear_cross_entropy(gt_ctx* ctx, float* loss, void* saved, vo
 extern "C" int gt_linear_topk_distillation(gt_ctx* ctx, float* loss, void* saved, void* scratch, const float* x, const float* w, const float* ids,
                                            const float* teacher, int64_t M, int64_t V, int64_t E, int64_t K, float temperature, int reduction,
                                            int precision) {
-  if (!ctx || !loss || !saved || !scratch || !x || !w || !ids || !teacher || bad_sizes(M, V, K) || bad_width(E) || bad_reduction(reduction) ||
-      bad_temperature(temperature) || bad_precision(precision)) return GT_ERR_INVALID_ARG;
+  if (!ctx || !loss || !saved || !scratch || !x || !w || !ids || !teacher || lm_bad_sizes(M, V, K) || bad_width(E) || lm_bad_reduction(reduction) ||
+      lm_bad_temperature(temperature) || bad_precision(precision)) return GT_ERR_INVALID_ARG;
   return linear_forward(ctx, loss, saved, scratch, x, w, nullptr, 0.0f, ids, teacher, M, V, E, K, temperature, reduction, precision);
 }
 
 extern "C" int gt_linear_loss_backward(gt_ctx* ctx, float* dx, float* dw, void* saved, void* scratch, const float* x, const float* w,
                                        const float* upstream, int64_t M, int64_t V, int64_t E, int64_t K, float temperature, int reduction,
                                        int precision, int acc_dx, int acc_dw) {
-  if (!ctx || !saved || !scratch || !x || !w || !upstream || bad_sizes(M, V, K) || bad_width(E) || bad_reduction(reduction) ||
-      bad_temperature(temperature) || bad_precision(precision)) return GT_ERR_INVALID_ARG;
+  if (!ctx || !saved || !scratch || !x || !w || !upstream || lm_bad_sizes(M, V, K) || bad_width(E) || lm_bad_reduction(reduction) ||
+      lm_bad_temperature(temperature) || bad_precision(precision)) return GT_ERR_INVALID_ARG;
   if (!dx && !dw) return GT_OK;
   Linear l = linear_layout(ctx, saved, scratch, M, V, E, K, precision);
   LmProblem& p = l.p;
@@ -621,39 +496,5 @@ extern "C" int gt_linear_loss_backward(gt_ctx* ctx, float* dx, float* dw, void* 
       ctx->launches += 1;
     }
   }
-  return GT_OK;
-}
-
-extern "C" int gt_topk_distillation_sizes(gt_ctx* ctx, int64_t B, int64_t C, int64_t K, size_t* saved) {
-  if (!ctx || !saved || bad_sizes(B, C, K)) return GT_ERR_INVALID_ARG;
-  *saved = saved_layout(nullptr, B, K).bytes + up256(sizeof(float) * B);
-  return GT_OK;
-}
-
-extern "C" int gt_topk_distillation(gt_ctx* ctx, float* loss, void* saved, const float* logits, int64_t ld_logits, const float* ids,
-                                    const float* teacher, int64_t B, int64_t C, int64_t K, float temperature, int reduction) {
-  if (!ctx || !loss || !saved || !logits || !ids || !teacher || bad_sizes(B, C, K) || ld_logits < C || bad_reduction(reduction) ||
-      bad_temperature(temperature)) return GT_ERR_INVALID_ARG;
-  const Saved s = saved_layout(saved, B, K);
-  float* rows = reduction == GT_REDUCE_NONE ? loss : (float*)((char*)saved + s.bytes);
-  int rc = prepare_targets(ctx, s, rows, nullptr, 0.0f, ids, teacher, B, C, K, temperature);
-  if (rc != GT_OK) return rc;
-  row_stats_kernel<<<(unsigned)B, 256, 0, ctx->stream>>>(logits, ld_logits, C, 1.0f / temperature, s.stats);
-  row_loss_kernel<<<(unsigned)((B + 7) / 8), 256, 0, ctx->stream>>>(rows, logits, ld_logits, B, (int)K, 1.0f / temperature, temperature, s);
-  GT_CUDA_OK(ctx, cudaGetLastError());
-  ctx->launches += 2;
-  return reduce_loss(ctx, loss, rows, B, reduction, s);
-}
-
-extern "C" int gt_topk_distillation_backward(gt_ctx* ctx, float* dlogits, int64_t ld_dlogits, void* saved, const float* logits, int64_t ld_logits,
-                                             const float* upstream, int64_t B, int64_t C, int64_t K, float temperature, int reduction,
-                                             int accumulate) {
-  if (!ctx || !dlogits || !saved || !logits || !upstream || bad_sizes(B, C, K) || ld_logits < C || ld_dlogits < C || bad_reduction(reduction) ||
-      bad_temperature(temperature)) return GT_ERR_INVALID_ARG;
-  const Saved s = saved_layout(saved, B, K);
-  row_grad_kernel<<<(unsigned)B, 256, 0, ctx->stream>>>(dlogits, ld_dlogits, logits, ld_logits, C, 1.0f / temperature, temperature, s, (int)K,
-                                                        upstream, reduction, accumulate);
-  GT_CUDA_OK(ctx, cudaGetLastError());
-  ctx->launches += 1;
   return GT_OK;
 }

@@ -4,14 +4,53 @@
 
 #include "gt_internal.h"
 
+constexpr int LM_TOP_MAX = 1024;             // targets of a row: they are sorted in shared memory
+constexpr int LM_UNUSED = 0x7fffffff;        // id of a place that is not in use; sorts behind every word
+
 // Values that a call computes on the device and later launches of it read.
 struct LmScalars {
   int count;            // rows that count
+  int done;             // blocks of a rows' kernel that have ended
   unsigned amax_x;      // largest finite |x|, |w| as float bits (whole-number maximum: the order does not matter)
   unsigned amax_w;
   float logit2;         // log2(e) / T times the operands' scales: accumulator -> z log2(e)
   float dx, dw;         // accumulator -> dx, dw
 };
+
+// What the forward pass leaves for the backward pass, in one block of memory.
+struct LmSaved {
+  LmScalars* scalars;
+  float* weight;    // by row: 1, or 0 for a row that does not count
+  float* konst;     // by row: sum of q log q
+  int* ids;         // (M, K), ascending, UNUSED at the end
+  float* q;         // (M, K), 0 where unused
+  int* row_of;      // rows that count, in order
+  float2* stats;    // (m, s): by row, m a logit (distillation of given logits); by compact row, m in units of log 2 (linear forms)
+  float2* factor;   // by compact row, see LmProblem
+  size_t bytes;
+};
+inline size_t lm_up256(size_t n) { return (n + 255) & ~(size_t)255; }
+struct LmCarve {
+  char* p; size_t at;
+  template <class T> T* take(size_t n) { T* r = (T*)(p + at); at += lm_up256(n * sizeof(T)); return r; }
+};
+inline LmSaved lm_saved(LmCarve& c, long long M, long long K) {
+  LmSaved s;
+  s.scalars = c.take<LmScalars>(1);
+  s.weight = c.take<float>(M);
+  s.konst = c.take<float>(M);
+  s.ids = c.take<int>(M * K);
+  s.q = c.take<float>(M * K);
+  s.row_of = c.take<int>(M);
+  s.stats = c.take<float2>(M);
+  s.factor = c.take<float2>(M);
+  s.bytes = c.at;
+  return s;
+}
+inline LmSaved lm_saved(void* base, long long M, long long K) {
+  LmCarve c = {(char*)base, 0};
+  return lm_saved(c, M, K);
+}
 
 // Two products' operands as 16-bit halves: v = 2^e (hi + lo), both fp16, scaled so that the matrix's largest value lies in
 // [2^14, 2^15).  Rows are `pitch` halves apart.
@@ -37,6 +76,16 @@ struct LmProblem {
 
 constexpr int LM_TILE = 256;     // rows and columns of the tile that a pair of CTAs computes
 constexpr int LM_KBLOCK = 64;    // k elements of one stage
+
+inline bool lm_bad_sizes(long long M, long long V, long long K) {      // ids are float-encoded: exact below 2^24
+  return M <= 0 || V <= 0 || K <= 0 || M > 0x7fffffff || V >= (1ll << 24) || K > LM_TOP_MAX;
+}
+inline bool lm_bad_temperature(float T) { return !(T > 0.0f) || T > 3.4e38f; }
+inline bool lm_bad_reduction(int r) { return r != GT_REDUCE_NONE && r != GT_REDUCE_MEAN && r != GT_REDUCE_SUM; }
+
+// Sorted targets, weights and the count of the rows of a distillation (top_targets_kernel); also 0 for the loss of rows that do not count.
+int gt_lm_top_targets(gt_ctx* ctx, const LmSaved& s, float* row_loss, const float* ids, const float* teacher, long long M, long long V, long long K,
+                      float T);
 
 // Forward: per row and half tile of words, (maximum, sum of exponentials).
 int gt_lm_stats(gt_ctx* ctx, const LmProblem& p);

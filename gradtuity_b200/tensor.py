@@ -1276,12 +1276,25 @@ class Tensor:
         out = empty_tensor((Bn,) if reduction == "none" else (1,))
         x_ptr, x_ld = self._rows()
         T = float(temperature)
-        _call("gt_topk_distillation", _vp(out.ptr), _vp(saved.ptr), _vp(x_ptr), x_ld, _vp(teacher_ids.ptr), _vp(teacher_logits.ptr), Bn, C, top, T, mode)
+        # As in cross_entropy: when the logits will need a gradient and have none yet, the loss kernel writes it in the same
+        # launch, for the upstream gradient of 1 that backward() seeds; another upstream gradient rescales it.
+        early = empty_padded_tensor(self.shape, x_ld) if self.requires_grad and self.grad is None and reduction != "none" else None
+        e_ptr, e_ld = early._rows() if early is not None else (0, 0)
+        _call("gt_topk_distillation", _vp(out.ptr), _vp(saved.ptr), _vp(e_ptr), e_ld, _vp(x_ptr), x_ld, _vp(teacher_ids.ptr), _vp(teacher_logits.ptr),
+              Bn, C, top, T, mode)
         logits = self
 
         def _backward(g: "Tensor") -> None:
+            nonlocal early
             if not logits.requires_grad:
                 return
+            if early is not None and logits.grad is None:
+                if not getattr(g, "_unit_seed", False):
+                    e_ptr, e_ld = early._rows()
+                    _call("gt_scale_by_device_scalar", _vp(e_ptr), _vp(g.ptr), Bn * e_ld)
+                logits.grad, early = early, None
+                return
+            early = None
             fresh = logits.grad is None
             if fresh:
                 # written, not accumulated; padded like the logits so that the products behind them read it by TMA

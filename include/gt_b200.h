@@ -417,10 +417,11 @@ int gt_linear_topk_distillation(gt_ctx* ctx, float* loss, void* saved, void* scr
 int gt_linear_loss_backward(gt_ctx* ctx, float* dx, float* dw, void* saved, void* scratch, const float* x, const float* w,
                             const float* upstream, int64_t M, int64_t V, int64_t E, int64_t K, float temperature, int reduction,
                             int precision, int acc_dx, int acc_dw);
-/* Distillation on given logits (B, C), rows ld floats apart.  saved: gt_topk_distillation_sizes bytes.                  */
+/* Distillation on given logits (B, C), rows ld floats apart.  saved: gt_topk_distillation_sizes bytes.  With dlogits given (not
+ * for GT_REDUCE_NONE) the same launch also writes the gradient for an upstream gradient of 1, as gt_cross_entropy_fused does. */
 int gt_topk_distillation_sizes(gt_ctx* ctx, int64_t B, int64_t C, int64_t K, size_t* saved);
-int gt_topk_distillation(gt_ctx* ctx, float* loss, void* saved, const float* logits, int64_t ld_logits, const float* ids,
-                         const float* teacher, int64_t B, int64_t C, int64_t K, float temperature, int reduction);
+int gt_topk_distillation(gt_ctx* ctx, float* loss, void* saved, float* dlogits, int64_t ld_dlogits, const float* logits, int64_t ld_logits,
+                         const float* ids, const float* teacher, int64_t B, int64_t C, int64_t K, float temperature, int reduction);
 int gt_topk_distillation_backward(gt_ctx* ctx, float* dlogits, int64_t ld_dlogits, void* saved, const float* logits, int64_t ld_logits,
                                   const float* upstream, int64_t B, int64_t C, int64_t K, float temperature, int reduction,
                                   int accumulate);

@@ -148,7 +148,7 @@ def test_entry_points_refuse_a_null_context():
     assert lib.gt_linear_topk_distillation(None, None, None, None, None, None, None, None, 1, 1, 1, 1, 1.0, 1, 0) == bad
     assert lib.gt_linear_loss_backward(None, None, None, None, None, None, None, None, 1, 1, 1, 1, 1.0, 1, 0, 0, 0) == bad
     assert lib.gt_topk_distillation_sizes(None, 1, 1, 1, byref(n)) == bad
-    assert lib.gt_topk_distillation(None, None, None, None, 1, None, None, 1, 1, 1, 1.0, 1) == bad
+    assert lib.gt_topk_distillation(None, None, None, None, 1, None, 1, None, None, 1, 1, 1, 1.0, 1) == bad
     assert lib.gt_topk_distillation_backward(None, None, 1, None, None, 1, None, 1, 1, 1, 1.0, 1, 0) == bad
 
 
@@ -162,7 +162,9 @@ def test_entry_points_refuse_bad_sizes(gt):
     p = c_void_p(256)          # never read: the call is refused first
     assert lib.gt_linear_cross_entropy(ctx, p, p, p, p, p, p, 5, 5, 5, -100.0, 3, 0) == gt.GT_ERR_INVALID_ARG
     assert lib.gt_linear_topk_distillation(ctx, p, p, p, p, p, p, p, 5, 5, 5, 1, ctypes.c_float(-1.0), 1, 0) == gt.GT_ERR_INVALID_ARG
-    assert lib.gt_topk_distillation(ctx, p, p, p, 4, p, p, 5, 5, 1, 1.0, 1) == gt.GT_ERR_INVALID_ARG       # pitch below the row length
+    assert lib.gt_topk_distillation(ctx, p, p, None, 0, p, 4, p, p, 5, 5, 1, 1.0, 1) == gt.GT_ERR_INVALID_ARG       # pitch below the row length
+    assert lib.gt_topk_distillation(ctx, p, p, p, 4, p, 5, p, p, 5, 5, 1, 1.0, 1) == gt.GT_ERR_INVALID_ARG
+    assert lib.gt_topk_distillation(ctx, p, p, p, 5, p, 5, p, p, 5, 5, 1, 1.0, 0) == gt.GT_ERR_INVALID_ARG          # gradient of 'none'
     assert lib.gt_linear_cross_entropy(ctx, p, p, p, p, p, p, 5, 5, 5, -100.0, 1, 7) == gt.GT_ERR_INVALID_ARG
 
 
