@@ -1,8 +1,8 @@
 // Distillation of given logits from a teacher's top logits (the formulas: gt_lmloss.cu): row kernels, bound by HBM.  A pass reads
 // the (rows, C) logits once and, with gradients, writes as much: 2 x 1.65 GB for 8192 rows of 50257 words.
 //
-// e^((z - m) / T) is 2^((z - m) log2(e) / T): z - m is exact where it matters and the formula holds for logits of any size, the
-// type's lowest value as a mask included.  Sums are in 32 bits; s and m are kept apart.
+// e^((z - m) / T) is 2^(z l2 - m l2) with l2 = log2(e) / T.  Sums are in 32 bits; s and m are kept apart, so that p carries no
+// rounding of a log-sum-exp.
 
 #include "gt_lmloss.h"
 
@@ -19,36 +19,58 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
-// A thread's running maximum and the sum of 2^((z - m) l2) beside it.  -inf adds nothing; a NaN ends up in the sum.
+// A thread's running maximum m and the sum of 2^(z l2 - m l2) beside it: one multiply-add and one ex2 per logit.  m starts at
+// LOW instead of -inf: words masked with -inf or with the type's lowest value then add 0 without a test.  A row whose logits are all
+// at LOW or below leaves (LOW, 0); it is summed again by `row_of_low_logits`.  A NaN ends up in the sum.
+constexpr float LOW = -1.0e30f;
 struct Running {
-  float m = -INFINITY, s = 0.0f;
+  float m = LOW, m2, s = 0.0f;
+  __device__ __forceinline__ explicit Running(float l2) { m2 = __fmul_rn(LOW, l2); }
   __device__ __forceinline__ void raise(float top, float l2) {
-    if (top > m) { s *= gt_ex2((m - top) * l2); m = top; }
+    if (top > m) { const float t2 = __fmul_rn(top, l2); s *= gt_ex2(m2 - t2); m = top; m2 = t2; }      // no fused residue: LOW l2 - LOW l2 is 0
   }
   __device__ __forceinline__ void add(float z, float l2) {
     raise(z, l2);
-    if (z != -INFINITY) s += gt_ex2((z - m) * l2);
+    s += gt_ex2(fmaf(z, l2, -m2));
   }
   __device__ __forceinline__ void add4(const float4& z, float l2) {
     raise(fmaxf(fmaxf(z.x, z.y), fmaxf(z.z, z.w)), l2);
-    const float e = (gt_ex2((z.x - m) * l2) + gt_ex2((z.y - m) * l2)) + (gt_ex2((z.z - m) * l2) + gt_ex2((z.w - m) * l2));
-    // -inf - -inf: nothing seen so far but masked words (a NaN among them is no maximum either, and counts)
-    if (m == -INFINITY) { s += (z.x == m ? 0.0f : z.x) + (z.y == m ? 0.0f : z.y) + (z.z == m ? 0.0f : z.z) + (z.w == m ? 0.0f : z.w); }
-    else s += e;
+    s += (gt_ex2(fmaf(z.x, l2, -m2)) + gt_ex2(fmaf(z.y, l2, -m2))) + (gt_ex2(fmaf(z.z, l2, -m2)) + gt_ex2(fmaf(z.w, l2, -m2)));
   }
 };
 
 // The block's (m, s) from its threads', in every thread: each warp leaves its own, and after a barrier each joins them all.
 __device__ __forceinline__ void leave_stats(const Running& r, float l2, float2* red) {
   const float m = warp_max(r.m);
-  const float s = warp_sum(r.m == -INFINITY ? r.s : r.s * gt_ex2((r.m - m) * l2));
+  const float s = warp_sum(r.s * gt_ex2(r.m2 - __fmul_rn(m, l2)));
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = make_float2(m, s);
 }
 __device__ __forceinline__ float2 join_stats(const float2* red, int warps, float l2) {
   const int l = threadIdx.x & 31;
-  const float2 a = l < warps ? red[l] : make_float2(-INFINITY, 0.0f);
+  const float2 a = l < warps ? red[l] : make_float2(LOW, 0.0f);
   const float m = warp_max(a.x);
-  const float s = warp_sum(a.x == -INFINITY ? a.y : a.y * gt_ex2((a.x - m) * l2));
+  const float s = warp_sum(a.y * gt_ex2(__fmul_rn(a.x, l2) - __fmul_rn(m, l2)));
+  return make_float2(m, s);
+}
+
+// (m, s) of a row without a logit above LOW, from global memory, by the whole block: the true maximum first, then differences.  All
+// words at -inf: (-inf, 0), and NaN from there on.
+__device__ __noinline__ float2 row_of_low_logits(const float* z, int C, float l2, float2* red, int warps) {
+  const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
+  float m = -INFINITY, s = 0.0f;
+  for (int j = threadIdx.x; j < C; j += blockDim.x) m = fmaxf(m, z[j]);
+  m = warp_max(m);
+  __syncthreads();
+  if (l == 0) red[w].x = m;
+  __syncthreads();
+  m = warp_max(l < warps ? red[l].x : -INFINITY);
+  if (m != -INFINITY)
+    for (int j = threadIdx.x; j < C; j += blockDim.x) s += gt_ex2((z[j] - m) * l2);
+  s = warp_sum(s);
+  __syncthreads();
+  if (l == 0) red[w].y = s;
+  __syncthreads();
+  s = warp_sum(l < warps ? red[l].y : 0.0f);
   return make_float2(m, s);
 }
 
@@ -127,7 +149,7 @@ __global__ void __launch_bounds__(STREAM_THREADS) distill_rows_kernel(const Rows
     if (BACKWARD) {
       st = p.s.stats[t];
     } else {
-      Running r;
+      Running r(p.l2);
 #pragma unroll 4
       for (int j = tid; j < body; j += STREAM_THREADS) r.add4(z4[j], p.l2);
       if (tid < head) r.add(z[tid], p.l2);
@@ -135,6 +157,7 @@ __global__ void __launch_bounds__(STREAM_THREADS) distill_rows_kernel(const Rows
       leave_stats(r, p.l2, red);
       __syncthreads();
       st = join_stats(red, STREAM_THREADS / 32, p.l2);
+      if (st.x == LOW && st.y == 0.0f) st = row_of_low_logits(z, p.C, p.l2, red, STREAM_THREADS / 32);
       if (tid < 32) {
         const float log_s = logf(st.y);
         float cross = 0.0f;
@@ -186,13 +209,14 @@ __global__ void __launch_bounds__(STREAM_THREADS) distill_rows_kernel(const Rows
 // gradient over it and the engine takes it out, chunk by chunk; a chunk of the next row is asked for as soon as the store of the
 // same chunk has been read out.  The row's up to three floats before its first 16-byte boundary and behind its last one are
 // read and written singly, so that any pitch will do.
-// Targets: a bit per 16 bytes of the row says whether one lies there, one word per warp and step; the thread that finds its bit set
-// searches the row's sorted ids, takes the targets' q off its gradient and leaves their logits for the loss.
+// Targets: thread k has the row's k-th, and a bit per word says that one lies there.  Between the passes the thread reads its
+// word's logit and writes its gradient; the second pass leaves words with a bit alone, so neither waits for the other.  (With
+// the second pass searching the sorted ids instead, 8192 x 50257 took 564 us with one target a row, 675 us with 32.)
 constexpr int ROW_THREADS = 1024;
 constexpr int ROW_MAX_CHUNKS = 14;
 constexpr int ROW_MAX_TOP = 256;
-constexpr int ROW_MIN_C = 4096, ROW_MAX_C = 54000;
-constexpr int ROW_MAP_WORDS = (ROW_MAX_C / 4 + 31) / 32 + 1;
+constexpr int ROW_MIN_C = 4096, ROW_MAX_C = 53248;
+constexpr int ROW_MAP_WORDS = ROW_MAX_C / 32 + 1;
 
 __device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
   uint32_t ok;
@@ -216,7 +240,7 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) distill_row_in_smem_kernel(con
   __shared__ double sums[32];
   __shared__ unsigned map[2][ROW_MAP_WORDS];
   __shared__ int top_id[2][ROW_MAX_TOP];
-  __shared__ float top_q[2][ROW_MAX_TOP], top_z[ROW_MAX_TOP];
+  __shared__ float top_q[2][ROW_MAX_TOP], cross_part[ROW_MAX_TOP / 32];
   __shared__ __align__(8) unsigned long long bars[ROW_MAX_CHUNKS];
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
@@ -259,55 +283,70 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) distill_row_in_smem_kernel(con
     const int edge = tid < head ? tid : tid >= 4 && tid < 8 && tail0 + tid - 4 < p.C ? tail0 + tid - 4 : -1;
     const float edge_z = edge >= 0 ? z[edge] : 0.0f;
     // ---- pass 1: running maximum and sum, chunk by chunk as they arrive
-    Running r;
+    Running r(p.l2);
     for (int c = 0; c < nchunks; ++c) {
       if (!bar_wait(bar0 + 8 * c, parity, abort_flag, status)) { ok = false; break; }       // leaves the chunk loop only
       const int u1 = min((c + 1) * q4, n4);
       for (int u = c * q4 + tid; u < u1; u += ROW_THREADS) r.add4(row4[u], p.l2);
     }
     if (edge >= 0) r.add(edge_z, p.l2);
-    // the targets' places, and those of the row before, which everybody is done with, off the other map
+    // the targets' bits (counted from `head`), and those of the row before, which everybody is done with, off the other map
     unsigned* const bits = map[it & 1];
+    const bool inside = my_id != LM_UNUSED && my_id >= head && my_id < tail0;
     if (tid < K) {
       const int old = top_id[(it & 1) ^ 1][tid], old_head = it > 0 ? head_of(row - gridDim.x) : 0;
-      if (old != LM_UNUSED && old >= old_head) map[(it & 1) ^ 1][(old - old_head) >> 7] = 0;
+      if (old != LM_UNUSED && old >= old_head) map[(it & 1) ^ 1][(old - old_head) >> 5] = 0;
       top_id[it & 1][tid] = my_id;
       top_q[it & 1][tid] = my_q;
-      if (my_id != LM_UNUSED && my_id >= head && my_id < tail0) {
-        const int u = (my_id - head) >> 2;
-        atomicOr(&bits[u >> 5], 1u << (u & 31));
-      }
+      if (inside) atomicOr(&bits[(my_id - head) >> 5], 1u << ((my_id - head) & 31));
     }
     leave_stats(r, p.l2, red);
     if (!__syncthreads_and(ok)) { ok = false; failed_parity = parity; break; }
-    const float2 st = join_stats(red, 32, p.l2);
-    const float c = weight != 0.0f ? c_row : 0.0f, f = c / st.y, m = st.x;
+    float2 st = join_stats(red, 32, p.l2);
+    if (st.x == LOW && st.y == 0.0f) st = row_of_low_logits(z, p.C, p.l2, red, 32);
+    const float c = c_row, m = st.x;
+    const bool live = weight != 0.0f;
+    // 2^(z l2 - m2) f in the second pass with the m2 of the first, whose rounding cancels in f = c / s; differences for logits
+    // whose product with l2 might overflow
+    const float m2 = __fmul_rn(m, p.l2), f = c / st.y;
+    const bool far = !(fabsf(m) < -LOW);
+    auto grad_of = [&](float x) { return f * gt_ex2(far ? (x - m) * p.l2 : fmaf(x, p.l2, -m2)); };
     const int* ids = top_id[it & 1];
     const float* qs = top_q[it & 1];
-    // g of the four words from `first` on, their logits x, with what targets among them take off
-    auto take_targets = [&](int first, const float4& x, float4& v) {
-      for (int lo = lower(ids, K, first); lo < K && ids[lo] < first + 4; ++lo) {
-        const int i = ids[lo] - first;
-        const float d = c * qs[lo];
-        if (i == 0) { v.x -= d; top_z[lo] = x.x; } else if (i == 1) { v.y -= d; top_z[lo] = x.y; }
-        else if (i == 2) { v.z -= d; top_z[lo] = x.z; } else { v.w -= d; top_z[lo] = x.w; }
+    float* const row_f = reinterpret_cast<float*>(row_smem);
+    if (tid < ROW_MAX_TOP) {                                    // whole warps
+      float cross = 0.0f;
+      if (my_id != LM_UNUSED && (tid == 0 || ids[tid - 1] != my_id)) {       // the first of a run of equal ids takes them all
+        float sum = my_q;
+        for (int k = tid + 1; k < K && ids[k] == my_id; ++k) sum += qs[k];
+        const float x = inside ? row_f[my_id - head] : z[my_id];
+        if (sum != 0.0f) cross = sum * ((x - m) / p.T - logf(st.y));
+        const float e = live ? grad_of(x) - c * sum : 0.0f;
+        if (inside) row_f[my_id - head] = e; else g[my_id] = e;
       }
-    };
+      cross = warp_sum(cross);
+      if ((tid & 31) == 0) cross_part[tid >> 5] = cross;
+    }
     // ---- pass 2: the gradient over the row, in place; each chunk leaves as soon as the whole block has written it
     if (edge >= 0) {
-      float e = f * gt_ex2((edge_z - m) * p.l2);
-      for (int k = lower(ids, K, edge); k < K && ids[k] == edge; ++k) { e -= c * qs[k]; top_z[k] = edge_z; }
-      g[edge] = weight != 0.0f ? e : 0.0f;
+      const int k = lower(ids, K, edge);
+      if (k == K || ids[k] != edge) g[edge] = live ? grad_of(edge_z) : 0.0f;
     }
     const long long next = row + gridDim.x;
     for (int c2 = 0; c2 < nchunks; ++c2) {
       const int u0 = c2 * q4, u1 = min(u0 + q4, n4);
       for (int u = u0 + tid; u < u1; u += ROW_THREADS) {
         const float4 x = row4[u];
-        float4 v = make_float4(f * gt_ex2((x.x - m) * p.l2), f * gt_ex2((x.y - m) * p.l2), f * gt_ex2((x.z - m) * p.l2), f * gt_ex2((x.w - m) * p.l2));
-        if ((bits[u >> 5] >> (u & 31)) & 1u) take_targets(head + 4 * u, x, v);
-        if (weight == 0.0f) v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        row4[u] = v;
+        const unsigned taken = bits[u >> 3] >> (4 * (u & 7)) & 15u;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (live && !far) v = make_float4(f * gt_ex2(fmaf(x.x, p.l2, -m2)), f * gt_ex2(fmaf(x.y, p.l2, -m2)), f * gt_ex2(fmaf(x.z, p.l2, -m2)),
+                                          f * gt_ex2(fmaf(x.w, p.l2, -m2)));
+        else if (live) v = make_float4(grad_of(x.x), grad_of(x.y), grad_of(x.z), grad_of(x.w));
+        if (taken == 0) { row4[u] = v; continue; }
+        if (!(taken & 1u)) row_f[4 * u] = v.x;
+        if (!(taken & 2u)) row_f[4 * u + 1] = v.y;
+        if (!(taken & 4u)) row_f[4 * u + 2] = v.z;
+        if (!(taken & 8u)) row_f[4 * u + 3] = v.w;
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncthreads();
@@ -326,18 +365,12 @@ __global__ void __launch_bounds__(ROW_THREADS, 1) distill_row_in_smem_kernel(con
       asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
       request(next, nchunks - 1);
     }
-    // the loss, from what the second pass found (the barrier of its last chunk lies between); the next row's second pass, which
-    // writes top_z again, is a barrier away
-    if (tid < 32 && weight != 0.0f) {
-      const float log_s = logf(st.y);
+    // the loss; a barrier of the second pass lies behind cross_part, another before it is written again
+    if (tid == 0 && live) {
       float cross = 0.0f;
-      for (int k = tid; k < K; k += 32)
-        if (qs[k] != 0.0f) cross += qs[k] * ((top_z[k] - m) / p.T - log_s);
-      cross = warp_sum(cross);
-      if (tid == 0) {
-        p.s.stats[row] = st;
-        p.row_loss[row] = p.T * p.T * (konst - cross);
-      }
+      for (int w = 0; w < ROW_MAX_TOP / 32; ++w) cross += cross_part[w];
+      p.s.stats[row] = st;
+      p.row_loss[row] = p.T * p.T * (konst - cross);
     }
   }
   if (tid == 0) {
