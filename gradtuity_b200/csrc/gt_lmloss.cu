@@ -230,40 +230,96 @@ __global__ void __launch_bounds__(256) split_kernel(const float* __restrict__ x,
 
 // ---- rows ------------------------------------------------------------------------------------------
 
-// The linear forms: joins the tiles' maxima and sums of a compact row, takes the logits of its targets in 32 bits straight from
-// x and w, and writes the row's loss.  A warp per row.
-__global__ void __launch_bounds__(256) linear_row_loss_kernel(float* __restrict__ row_loss, const float2* __restrict__ partial, int parts,
-                                                              const float* __restrict__ x, const float* __restrict__ w, long long M, long long E,
-                                                              int K, float T, LmSaved s) {
-  const long long i = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int l = threadIdx.x & 31;
-  if (i >= s.scalars->count) return;
+// The linear forms: (m, s) of the rows that count from the parts' (tiles of words, or blocks).  32 rows a block, their parts shared
+// out over the warps, so that a warp reads whole lines.  by_row: parts and stats go by row, not by compact row.
+__global__ void __launch_bounds__(256) join_stats_kernel(const float2* __restrict__ partial, int parts, long long M, int by_row, LmSaved s) {
+  __shared__ float2 red[8][32];
+  const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
+  const long long i = (long long)blockIdx.x * 32 + l;
+  const bool live = i < s.scalars->count;
+  const long long at = live && by_row ? s.row_of[i] : i;
   float m = -INFINITY, sum = 0.0f;                            // m in units of log 2
-  for (int j = l; j < parts; j += 32) {
-    const float2 b = partial[(long long)j * M + i];
+  auto add = [&](float2 b) {
     const float top = fmaxf(m, b.x);
-    if (top == -INFINITY) { sum += b.y; continue; }
+    if (top == -INFINITY) { sum += b.y; return; }             // nothing but words that do not exist; or a NaN, which counts
     sum = sum * gt_ex2(m - top) + b.y * gt_ex2(b.x - top);
     m = top;
+  };
+  if (live) {
+#pragma unroll 4
+    for (int j = w; j < parts; j += 8) add(partial[(long long)j * M + at]);
   }
-  const float top = warp_max(m);
-  sum = warp_sum(top == -INFINITY ? sum : sum * gt_ex2(m - top));
-  const long long t = s.row_of[i];
-  const float log_s = logf(sum), mean = top * 0.6931471805599453f;
+  red[w][l] = make_float2(m, sum);
+  __syncthreads();
+  if (w != 0 || !live) return;
+  for (int k = 1; k < 8; ++k) add(red[k][l]);
+  s.stats[at] = make_float2(m, sum);
+}
+
+// Losses of the compact rows, from the logits of their targets, taken in 32 bits straight from x and w.  WARPS_A_ROW warps share a
+// row's targets.  The last block to end adds the rows' losses up, in 64 bits and in a fixed order.
+template <int WARPS_A_ROW>
+__global__ void __launch_bounds__(256) target_loss_kernel(float* __restrict__ row_loss, float* __restrict__ loss, const float* __restrict__ x,
+                                                          const float* __restrict__ w, long long M, int E, int K, float T, int mean, int by_row, LmSaved s) {
+  __shared__ float part[8];
+  __shared__ double sums[8];
+  __shared__ int last;
+  const int warp = threadIdx.x >> 5, l = threadIdx.x & 31;
+  const long long i = (long long)blockIdx.x * (8 / WARPS_A_ROW) + warp / WARPS_A_ROW;
+  const bool live = i < s.scalars->count;
+  long long t = 0;
   float cross = 0.0f;
-  for (int k = 0; k < K; ++k) {
-    const int id = s.ids[t * K + k];
-    if (id == LM_UNUSED) break;
-    const float q = s.q[t * K + k];
-    if (q == 0.0f) continue;
-    float z = 0.0f;
-    for (long long e = l; e < E; e += 32) z = fmaf(x[t * E + e], w[(long long)id * E + e], z);
-    z = warp_sum(z) / T;
-    cross += q * ((z - mean) - log_s);
+  if (live) {
+    t = s.row_of[i];
+    const float2 st = s.stats[by_row ? t : i];
+    const float log_s = logf(st.y), top = st.x * 0.6931471805599453f;
+    const float* xr = x + t * E;
+    const bool vec = ((uintptr_t)x & 15) == 0 && ((uintptr_t)w & 15) == 0 && E % 4 == 0;
+    for (int k = warp % WARPS_A_ROW; k < K; k += WARPS_A_ROW) {
+      const int id = s.ids[t * K + k];
+      if (id == LM_UNUSED) break;
+      const float q = s.q[t * K + k];
+      if (q == 0.0f) continue;
+      const float* wr = w + (long long)id * E;
+      float z = 0.0f;
+      if (vec) {
+#pragma unroll 4
+        for (int e = 4 * l; e < E; e += 128) {
+          const float4 a = *reinterpret_cast<const float4*>(xr + e), b = *reinterpret_cast<const float4*>(wr + e);
+          z = fmaf(a.x, b.x, z); z = fmaf(a.y, b.y, z); z = fmaf(a.z, b.z, z); z = fmaf(a.w, b.w, z);
+        }
+      } else {
+#pragma unroll 4
+        for (int e = l; e < E; e += 32) z = fmaf(xr[e], wr[e], z);
+      }
+      z = warp_sum(z) / T;
+      cross += q * ((z - top) - log_s);
+    }
   }
-  if (l == 0) {
-    s.stats[i] = make_float2(top, sum);
-    row_loss[t] = T * T * (s.konst[t] - cross);
+  if (WARPS_A_ROW > 1) {
+    if (l == 0) part[warp] = cross;
+    __syncthreads();
+    cross = 0.0f;
+    for (int k = 0; k < WARPS_A_ROW; ++k) cross += part[warp / WARPS_A_ROW * WARPS_A_ROW + k];
+  }
+  if (live && l == 0 && warp % WARPS_A_ROW == 0) row_loss[t] = T * T * (s.konst[t] - cross);
+  if (!loss) return;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(&s.scalars->done, 1) == (int)gridDim.x - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  double a = 0.0;
+  for (long long r = threadIdx.x; r < M; r += 256) a += __ldcg(row_loss + r);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+  if (l == 0) sums[warp] = a;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int k = 1; k < 8; ++k) a += sums[k];
+    if (mean && s.scalars->count > 0) a /= (double)s.scalars->count;
+    *loss = (float)a;
   }
 }
 
@@ -318,23 +374,6 @@ __global__ void __launch_bounds__(256) add_shares_kernel(float* __restrict__ dx,
   }
 }
 
-// Sum or mean of the rows' losses in 64 bits, in a fixed order: one block.
-__global__ void __launch_bounds__(1024) reduce_loss_kernel(float* __restrict__ loss, const float* __restrict__ row_loss, long long M, const int* count,
-                                                           int mean) {
-  __shared__ double part[32];
-  double a = 0.0;
-  for (long long t = threadIdx.x; t < M; t += 1024) a += row_loss[t];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = a;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < 32; ++w) a += part[w];
-    if (mean && *count > 0) a /= (double)*count;
-    *loss = (float)a;
-  }
-}
-
 bool bad_width(long long E) { return E <= 0 || E > (1 << 24); }
 
 bool bad_precision(int p) { return p != GT_PREC_TF32 && p != GT_PREC_TF32X3 && p != GT_PREC_FP32; }
@@ -344,6 +383,8 @@ struct Linear {
   LmSaved s;
   LmProblem p;
   float* row_loss;
+  float* dx_part;                  // few rows
+  bool few_rows;
   int pieces;
   size_t saved_bytes, scratch_bytes;
 };
@@ -352,6 +393,18 @@ Linear linear_layout(gt_ctx* ctx, void* saved, void* scratch, long long M, long 
   memset(&l, 0, sizeof(l));
   LmProblem& p = l.p;
   p.M = M; p.V = V; p.E = E; p.K = (int)K;
+  l.few_rows = gt_lm_few_rows(M, V, E);
+  if (l.few_rows) {
+    LmCarve c = {(char*)saved, 0}, f = {(char*)scratch, 0};
+    l.s = lm_saved(c, M, K);
+    l.saved_bytes = c.at;
+    LmCarve b = f;
+    l.row_loss = f.take<float>(M);
+    p.partial = f.take<float2>((size_t)gt_lm_rows_parts(ctx, M, V, false) * M);
+    l.dx_part = b.take<float>((size_t)gt_lm_rows_parts(ctx, M, V, true) * M * E);
+    l.scratch_bytes = f.at > b.at ? f.at : b.at;
+    return l;
+  }
   p.products = precision == GT_PREC_TF32 ? 1 : 3;
   p.pitch_e = (E + 7) / 8 * 8;
   // Words of a piece: what PIECE_BYTES hold of G for M rows (two pieces of it exist at a time), in whole tiles.
@@ -388,6 +441,14 @@ Linear linear_layout(gt_ctx* ctx, void* saved, void* scratch, long long M, long 
   return l;
 }
 
+LmRows rows_problem(const Linear& l, const float* x, const float* w, long long M, long long V, long long E, long long K, float T, int reduction) {
+  LmRows r;
+  memset(&r, 0, sizeof(r));
+  r.M = (int)M; r.V = (int)V; r.E = (int)E; r.K = (int)K;
+  r.x = x; r.w = w; r.T = T; r.s = l.s; r.partial = l.p.partial; r.reduction = reduction;
+  return r;
+}
+
 int prepare_linear(gt_ctx* ctx, const LmSaved& s, float* row_loss, const float* targets, float ignore, const float* ids, const float* teacher,
                     long long M, long long V, long long K, float T) {
   if (targets) {
@@ -404,11 +465,15 @@ int prepare_linear(gt_ctx* ctx, const LmSaved& s, float* row_loss, const float* 
   return GT_OK;
 }
 
-int reduce_loss(gt_ctx* ctx, float* loss, const float* row_loss, long long M, int reduction, const LmSaved& s) {
-  if (reduction == GT_REDUCE_NONE) return GT_OK;
-  reduce_loss_kernel<<<1, 1024, 0, ctx->stream>>>(loss, row_loss, M, &s.scalars->count, reduction == GT_REDUCE_MEAN);
+int finish_rows(gt_ctx* ctx, float* row_loss, float* loss, const float2* partial, int parts, const float* x, const float* w, long long M,
+                long long E, long long K, float T, int reduction, int by_row, const LmSaved& s) {
+  float* out = reduction == GT_REDUCE_NONE ? nullptr : loss;
+  const int mean = reduction == GT_REDUCE_MEAN;
+  join_stats_kernel<<<(unsigned)((M + 31) / 32), 256, 0, ctx->stream>>>(partial, parts, M, by_row, s);
+  if (K == 1) target_loss_kernel<1><<<(unsigned)((M + 7) / 8), 256, 0, ctx->stream>>>(row_loss, out, x, w, M, (int)E, (int)K, T, mean, by_row, s);
+  else target_loss_kernel<8><<<(unsigned)M, 256, 0, ctx->stream>>>(row_loss, out, x, w, M, (int)E, (int)K, T, mean, by_row, s);
   GT_CUDA_OK(ctx, cudaGetLastError());
-  ctx->launches += 1;
+  ctx->launches += 2;
   return GT_OK;
 }
 
@@ -417,6 +482,20 @@ int linear_forward(gt_ctx* ctx, float* loss, void* saved, void* scratch, const f
   const Linear l = linear_layout(ctx, saved, scratch, M, V, E, K, precision);
   const LmSaved& s = l.s;
   float* rows = reduction == GT_REDUCE_NONE ? loss : l.row_loss;
+  if (l.few_rows) {
+    LmRows r = rows_problem(l, x, w, M, V, E, K, T, reduction);
+    r.parts = gt_lm_rows_parts(ctx, M, V, false);
+    if (!targets) {
+      int rc = prepare_linear(ctx, s, rows, nullptr, 0.0f, ids, teacher, M, V, K, T);
+      if (rc == GT_OK) rc = gt_lm_rows_forward(ctx, r);
+      return rc != GT_OK ? rc : finish_rows(ctx, rows, loss, l.p.partial, r.parts, x, w, M, E, K, T, reduction, 1, s);
+    }
+    GT_CUDA_OK(ctx, cudaMemsetAsync(s.scalars, 0, sizeof(LmScalars), ctx->stream));
+    r.targets = targets; r.ignore = ignore;
+    r.row_loss = rows;
+    r.loss = reduction == GT_REDUCE_NONE ? nullptr : loss;
+    return gt_lm_rows_forward(ctx, r);
+  }
   int rc = prepare_linear(ctx, s, rows, targets, ignore, ids, teacher, M, V, K, T);
   if (rc != GT_OK) return rc;
   GT_CUDA_OK(ctx, cudaMemsetAsync(l.p.counters, 0, sizeof(int), ctx->stream));
@@ -429,10 +508,7 @@ int linear_forward(gt_ctx* ctx, float* loss, void* saved, void* scratch, const f
   ctx->launches += 2;
   rc = gt_lm_stats(ctx, l.p);
   if (rc != GT_OK) return rc;
-  linear_row_loss_kernel<<<(unsigned)((M + 7) / 8), 256, 0, ctx->stream>>>(rows, l.p.partial, (int)((V + LM_TILE - 1) / LM_TILE * 2), x, w, M, E, (int)K, T, s);
-  GT_CUDA_OK(ctx, cudaGetLastError());
-  ctx->launches += 1;
-  return reduce_loss(ctx, loss, rows, M, reduction, s);
+  return finish_rows(ctx, rows, loss, l.p.partial, (int)((V + LM_TILE - 1) / LM_TILE * 2), x, w, M, E, K, T, reduction, 0, s);
 }
 
 }  // namespace
@@ -476,6 +552,13 @@ extern "C" int gt_linear_loss_backward(gt_ctx* ctx, float* dx, float* dw, void* 
       lm_bad_temperature(temperature) || bad_precision(precision)) return GT_ERR_INVALID_ARG;
   if (!dx && !dw) return GT_OK;
   Linear l = linear_layout(ctx, saved, scratch, M, V, E, K, precision);
+  if (l.few_rows) {
+    LmRows r = rows_problem(l, x, w, M, V, E, K, temperature, reduction);
+    r.parts = gt_lm_rows_parts(ctx, M, V, true);
+    r.upstream = upstream; r.dw = dw; r.acc_dw = acc_dw;
+    r.dx_part = dx ? l.dx_part : nullptr;
+    return gt_lm_rows_backward(ctx, r, dx, acc_dx);
+  }
   LmProblem& p = l.p;
   p.dx = dx; p.dw = dw; p.acc_dx = acc_dx; p.acc_dw = acc_dw;
   GT_CUDA_OK(ctx, cudaMemsetAsync(p.counters, 0, sizeof(int) * (l.pieces + 1), ctx->stream));

@@ -93,3 +93,23 @@ int gt_lm_stats(gt_ctx* ctx, const LmProblem& p);
 int gt_lm_step(gt_ctx* ctx, const LmProblem& p, int piece);
 // Pairs of CTAs that run at the same time; 0 when the query fails.
 int gt_lm_pairs(gt_ctx* ctx);
+
+// ---- few rows, or little work (gt_lmloss_rows.cu) ----
+struct LmRows {
+  int M, V, E, K;
+  const float* x; const float* w;
+  float T;
+  const float* targets; float ignore;      // cross entropy: the forward kernel takes the losses itself
+  LmSaved s;
+  float2* partial;                         // (parts, M)
+  int parts;                               // blocks over the words
+  float* row_loss; float* loss;            // either may be null
+  const float* upstream; int reduction;
+  float* dw; int acc_dw;
+  float* dx_part;                          // (parts, M, E); null: no dx wanted
+};
+constexpr long long LM_ROWS_WORK = 64ll << 20;
+bool gt_lm_few_rows(long long M, long long V, long long E);
+int gt_lm_rows_parts(gt_ctx* ctx, long long M, long long V, bool backward);
+int gt_lm_rows_forward(gt_ctx* ctx, const LmRows& p);
+int gt_lm_rows_backward(gt_ctx* ctx, const LmRows& p, float* dx, int acc_dx);

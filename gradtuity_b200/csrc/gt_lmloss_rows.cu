@@ -1,0 +1,376 @@
+// The linear losses (gt_lmloss.cu) for few rows, or for little work, in 32-bit multiply-adds: what a row or a few cost is reading W
+// (and writing dW), and a small problem is launches and latencies; the tensor-core path pays for splitting W into halves first,
+// and for tiles of 256 rows.
+//
+// A block of eight warps takes 32 words at a time.  The E columns are shared out over its lanes, C of them each, and MT rows of x stay
+// in registers; every lane multiplies its columns of a few words with its columns of the rows, the 32 lanes add up by exchanging
+// halves (one exchange per value instead of five), and the warps' sums meet in shared memory.  So W is read once, straight from
+// memory in whole lines, and no operand passes through shared memory.
+// Forward: running maximum and sum of each row; the last block to end joins the blocks' and, for cross entropy, takes the losses.
+// Backward: the logits again, G = c (p - q), then from the same words dx += G w (in registers, one partial sum per block, added up
+// in the blocks' order by a second kernel) and dW = G^T x, written straight out.
+// More than MT rows: the rows' tiles one after the other, adding to dW.
+
+#include "gt_lmloss.h"
+
+namespace {
+
+constexpr int THREADS = 256, WARPS = 8, WORDS = 32;
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// N values per lane, a power of two up to 64, summed over the lanes: afterwards lane l holds the sums max(1, N / 32) l .. (N >= 32),
+// or the sum l N / 32 (N < 32).
+template <int N>
+__device__ __forceinline__ void lanes_sum(float (&v)[N]) {
+  const int lane = threadIdx.x & 31;
+  int n = N;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    if (n > 1) {
+      n >>= 1;
+      const bool up = (lane & o) != 0;
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) {
+        if (i < n) {
+          const float send = up ? v[i] : v[i + n], keep = up ? v[i + n] : v[i];
+          v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+        }
+      }
+    } else {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+    }
+  }
+}
+
+template <int MT> struct Words { static constexpr int N = MT == 1 ? 16 : MT == 4 ? 8 : 4; };     // words multiplied at a time
+
+struct Rows {
+  LmRows r;
+  int* status;
+};
+
+// The block's logits of 32 words and MT rows: each warp leaves its columns' share in red[warp][row][word].
+template <int MT, int C>
+__device__ __forceinline__ void dots(const float (&x)[MT][C], const float* __restrict__ w, long long v0, int V, int E, int col0, float* red) {
+  constexpr int WS = Words<MT>::N;
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int s = 0; s < WORDS; s += WS) {
+    float b[WS][C];
+#pragma unroll
+    for (int i = 0; i < WS; ++i)
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int col = col0 + 32 * c;
+        b[i][c] = v0 + s + i < V && col < E ? w[(v0 + s + i) * E + col] : 0.0f;
+      }
+    float a[WS * MT];
+#pragma unroll
+    for (int i = 0; i < WS; ++i)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        float t = 0.0f;
+#pragma unroll
+        for (int c = 0; c < C; ++c) t = fmaf(x[m][c], b[i][c], t);
+        a[i * MT + m] = t;
+      }
+    lanes_sum<WS * MT>(a);
+    constexpr int PER = WS * MT / 32 > 0 ? WS * MT / 32 : 1;
+    if (WS * MT >= 32 || (lane & (32 / (WS * MT > 32 ? 32 : WS * MT) - 1)) == 0) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        const int at = WS * MT >= 32 ? lane * PER + j : lane * (WS * MT) / 32;
+        red[(at % MT) * WORDS + s + at / MT] = a[j];
+      }
+    }
+  }
+}
+
+template <int MT, int C>
+__device__ __forceinline__ void load_rows(float (&x)[MT][C], const float* __restrict__ src, int m0, int M, int E, int col0, const float* weight) {
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const bool row = m0 + m < M && (weight == nullptr || weight[m0 + m] != 0.0f);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int col = col0 + 32 * c;
+      x[m][c] = row && col < E ? src[(long long)(m0 + m) * E + col] : 0.0f;
+    }
+  }
+}
+
+// Row t's (m log2 e, s) from the blocks' partial ones, by a warp.
+__device__ __forceinline__ float2 join_parts(const float2* partial, int parts, long long M, long long t) {
+  float m = -INFINITY, s = 0.0f;
+  for (int j = threadIdx.x & 31; j < parts; j += 32) {
+    const float2 b = __ldcg(partial + (long long)j * M + t);
+    const float top = fmaxf(m, b.x);
+    if (top == -INFINITY) { s += b.y; continue; }
+    s = s * gt_ex2(m - top) + b.y * gt_ex2(b.x - top);
+    m = top;
+  }
+  const float top = warp_max(m);
+  s = warp_sum(top == -INFINITY ? s : s * gt_ex2(m - top));
+  return make_float2(top, s);
+}
+
+template <int MT, int C>
+__global__ void __launch_bounds__(THREADS) few_rows_forward_kernel(const Rows a) {
+  const LmRows& p = a.r;
+  __shared__ float red[2][WARPS][MT * WORDS];
+  __shared__ int last;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int active = (p.E + 32 * C - 1) / (32 * C);             // warps that have columns
+  const int col0 = warp * 32 * C + lane, m0 = blockIdx.y * MT;
+  float x[MT][C];
+  load_rows<MT, C>(x, p.x, m0, p.M, p.E, col0, nullptr);
+  constexpr int ROWS = (MT + WARPS - 1) / WARPS;                // rows whose maximum and sum a warp keeps
+  float m[ROWS], s[ROWS];
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) { m[i] = -INFINITY; s[i] = 0.0f; }
+  const float l2 = 1.4426950408889634f / p.T;
+  int buf = 0;
+  for (long long v0 = (long long)blockIdx.x * WORDS; v0 < p.V; v0 += (long long)gridDim.x * WORDS, buf ^= 1) {
+    if (warp < active) dots<MT, C>(x, p.w, v0, p.V, p.E, col0, red[buf][warp]);
+    __syncthreads();                                            // the other buffer is free: its readers passed this barrier
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const int r = warp + i * WARPS;
+      if (r < MT) {
+        float z = 0.0f;
+        for (int k = 0; k < active; ++k) z += red[buf][k][r * WORDS + lane];
+        z = v0 + lane < p.V ? z * l2 : -INFINITY;
+        const float top = fmaxf(m[i], warp_max(z));
+        if (top != -INFINITY) {
+          s[i] = s[i] * gt_ex2(m[i] - top) + warp_sum(gt_ex2(z - top));
+          m[i] = top;
+        } else {
+          s[i] += warp_sum(z == -INFINITY ? 0.0f : z);          // a NaN is no maximum, but it counts
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    const int r = warp + i * WARPS;
+    if (r < MT && m0 + r < p.M && lane == 0) p.partial[(long long)blockIdx.x * p.M + m0 + r] = make_float2(m[i], s[i]);
+  }
+  if (!p.targets) return;                                       // distillation: the rows' kernels do the rest
+
+  // ---- cross entropy: the last block takes the losses
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(&p.s.scalars->done, 1) == (int)(gridDim.x * gridDim.y) - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  double total = 0.0;
+  int n = 0;
+  for (int t = warp; t < p.M; t += WARPS) {
+    const float f = p.targets[t];
+    const bool in_range = f >= 0.0f && f < (float)p.V, used = f != p.ignore && in_range;
+    float loss = 0.0f;
+    if (used) {
+      const float2 st = join_parts(p.partial, gridDim.x, p.M, t);
+      const int id = (int)f;
+      float z = 0.0f;
+      for (int e = lane; e < p.E; e += 32) z = fmaf(p.x[(long long)t * p.E + e], p.w[(long long)id * p.E + e], z);
+      z = warp_sum(z);
+      loss = logf(st.y) - (z - st.x * 0.6931471805599453f);
+      if (lane == 0) p.s.stats[t] = st;
+      total += loss;
+      ++n;
+    }
+    if (lane == 0) {
+      if (f != p.ignore && !in_range) atomicExch(a.status, GT_ERR_INVALID_ARG);
+      p.s.ids[t] = used ? (int)f : LM_UNUSED;
+      p.s.q[t] = used ? 1.0f : 0.0f;
+      p.s.weight[t] = used ? 1.0f : 0.0f;
+      if (p.row_loss) p.row_loss[t] = loss;
+    }
+  }
+  __shared__ double totals[WARPS];
+  __shared__ int counts[WARPS];
+  if (lane == 0) { totals[warp] = total; counts[warp] = n; }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int k = 1; k < WARPS; ++k) { total += totals[k]; n += counts[k]; }
+    p.s.scalars->count = n;
+    if (p.loss) *p.loss = (float)(p.reduction == GT_REDUCE_MEAN && n > 0 ? total / n : total);
+  }
+}
+
+template <int MT, int C>
+__global__ void __launch_bounds__(THREADS) few_rows_backward_kernel(const Rows a) {
+  const LmRows& p = a.r;
+  __shared__ float red[WARPS][MT * WORDS];
+  __shared__ __align__(16) float gs[WORDS * MT];                // G, word by word
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int active = (p.E + 32 * C - 1) / (32 * C);
+  const int col0 = warp * 32 * C + lane;
+  const float l2 = 1.4426950408889634f / p.T;
+  constexpr int ROWS = (MT + WARPS - 1) / WARPS;
+  for (int m0 = 0; m0 < p.M; m0 += MT) {
+    float x[MT][C], dx[MT][C];
+    load_rows<MT, C>(x, p.x, m0, p.M, p.E, col0, p.s.weight);
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int c = 0; c < C; ++c) dx[m][c] = 0.0f;
+    // the rows whose G this warp makes
+    float top[ROWS], f[ROWS], cq[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const int t = m0 + warp + i * WARPS;
+      top[i] = 0.0f; f[i] = 0.0f; cq[i] = 0.0f;
+      if (warp + i * WARPS < MT && t < p.M && p.s.weight[t] != 0.0f) {
+        float c = p.T * (p.reduction == GT_REDUCE_NONE ? p.upstream[t] : p.upstream[0]);
+        if (p.reduction == GT_REDUCE_MEAN) c /= (float)p.s.scalars->count;
+        const float2 st = p.s.stats[t];
+        top[i] = st.x; f[i] = c / st.y; cq[i] = c;
+      }
+    }
+    for (long long v0 = (long long)blockIdx.x * WORDS; v0 < p.V; v0 += (long long)gridDim.x * WORDS) {
+      if (warp < active) dots<MT, C>(x, p.w, v0, p.V, p.E, col0, red[warp]);
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) {
+        const int r = warp + i * WARPS;
+        if (r < MT) {
+          float z = 0.0f;
+          for (int k = 0; k < active; ++k) z += red[k][r * WORDS + lane];
+          const int t = m0 + r, v = (int)v0 + lane;
+          float g = 0.0f;
+          if (t < p.M && p.s.weight[t] != 0.0f && v < p.V) {
+            g = f[i] * gt_ex2(z * l2 - top[i]);
+            const int* ids = p.s.ids + (long long)t * p.K;
+            int lo = 0, hi = p.K;                               // the row's targets at this word
+            while (lo < hi) { const int mid = (lo + hi) >> 1; if (ids[mid] < v) lo = mid + 1; else hi = mid; }
+            for (; lo < p.K && ids[lo] == v; ++lo) g -= cq[i] * p.s.q[(long long)t * p.K + lo];
+          }
+          gs[lane * MT + r] = g;
+        }
+      }
+      __syncthreads();
+      if (warp < active) {
+#pragma unroll 4
+        for (int i = 0; i < WORDS; ++i) {
+          float g[MT];
+          if (MT >= 4) {
+#pragma unroll
+            for (int m = 0; m < MT; m += 4) *reinterpret_cast<float4*>(g + m) = *reinterpret_cast<const float4*>(gs + i * MT + m);
+          } else {
+            g[0] = gs[i];
+          }
+          const long long v = v0 + i;
+          if (v >= p.V) break;
+#pragma unroll
+          for (int c = 0; c < C; ++c) {
+            const int col = col0 + 32 * c;
+            if (col >= p.E) continue;
+            if (p.dx_part) {
+              const float b = p.w[v * p.E + col];               // read a moment ago: in L1
+#pragma unroll
+              for (int m = 0; m < MT; ++m) dx[m][c] = fmaf(g[m], b, dx[m][c]);
+            }
+            if (p.dw) {
+              float d = p.acc_dw || m0 > 0 ? p.dw[v * p.E + col] : 0.0f;
+#pragma unroll
+              for (int m = 0; m < MT; ++m) d = fmaf(g[m], x[m][c], d);
+              p.dw[v * p.E + col] = d;
+            }
+          }
+        }
+      }
+      // gs is written again behind the next block's first barrier; red behind this block's second one
+    }
+    if (p.dx_part && warp < active) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          const int col = col0 + 32 * c;
+          if (m0 + m < p.M && col < p.E) p.dx_part[((long long)blockIdx.x * p.M + m0 + m) * p.E + col] = dx[m][c];
+        }
+    }
+  }
+}
+
+// dx (+)= the blocks' shares in their order: 32 columns of a row per block, the warps take every eighth share.
+__global__ void __launch_bounds__(THREADS) few_rows_dx_kernel(float* __restrict__ dx, const float* __restrict__ part, int parts, long long M, int E, int add) {
+  __shared__ float sums[WARPS][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int col = blockIdx.x * 32 + lane;
+  const long long t = blockIdx.y;
+  float s = 0.0f;
+  if (col < E) {
+#pragma unroll 8
+    for (int j = warp; j < parts; j += WARPS) s += part[((long long)j * M + t) * E + col];
+  }
+  sums[warp][lane] = s;
+  __syncthreads();
+  if (warp == 0 && col < E) {
+    for (int k = 1; k < WARPS; ++k) s += sums[k][lane];
+    dx[t * E + col] = add ? dx[t * E + col] + s : s;
+  }
+}
+
+template <int MT, int C>
+int launch_as(gt_ctx* ctx, const Rows& a, bool backward) {
+  const LmRows& p = a.r;
+  if (backward) few_rows_backward_kernel<MT, C><<<(unsigned)p.parts, THREADS, 0, ctx->stream>>>(a);
+  else few_rows_forward_kernel<MT, C><<<dim3((unsigned)p.parts, (unsigned)((p.M + MT - 1) / MT)), THREADS, 0, ctx->stream>>>(a);
+  GT_CUDA_OK(ctx, cudaGetLastError());
+  ctx->launches += 1;
+  return GT_OK;
+}
+template <int MT>
+int launch_for(gt_ctx* ctx, const Rows& a, bool backward) {
+  switch ((a.r.E + 255) / 256) {
+    case 1: return launch_as<MT, 1>(ctx, a, backward);
+    case 2: return launch_as<MT, 2>(ctx, a, backward);
+    case 3: return launch_as<MT, 3>(ctx, a, backward);
+    default: return launch_as<MT, 4>(ctx, a, backward);
+  }
+}
+int launch(gt_ctx* ctx, const LmRows& p, bool backward) {
+  const Rows a = {p, ctx->d_status};
+  if (p.M == 1) return launch_for<1>(ctx, a, backward);
+  if (p.M <= 4) return launch_for<4>(ctx, a, backward);
+  return launch_for<16>(ctx, a, backward);
+}
+
+}  // namespace
+
+bool gt_lm_few_rows(long long M, long long V, long long E) {
+  if (E > 1024) return false;
+  return M <= 16 || (M <= 256 && M * V * E <= LM_ROWS_WORK);
+}
+
+int gt_lm_rows_parts(gt_ctx* ctx, long long M, long long V, bool backward) {
+  const long long blocks = (V + WORDS - 1) / WORDS, tiles = M <= 16 ? 1 : (M + 15) / 16;
+  long long most = 2ll * ctx->sm_count;                          // two blocks an SM
+  if (!backward) most = (most + tiles - 1) / tiles;
+  return (int)(blocks < most ? blocks : most);
+}
+
+int gt_lm_rows_forward(gt_ctx* ctx, const LmRows& p) { return launch(ctx, p, false); }
+
+int gt_lm_rows_backward(gt_ctx* ctx, const LmRows& p, float* dx, int acc_dx) {
+  int rc = launch(ctx, p, true);
+  if (rc != GT_OK || !dx) return rc;
+  few_rows_dx_kernel<<<dim3((unsigned)((p.E + 31) / 32), (unsigned)p.M), THREADS, 0, ctx->stream>>>(dx, p.dx_part, p.parts, p.M, p.E, acc_dx);
+  GT_CUDA_OK(ctx, cudaGetLastError());
+  ctx->launches += 1;
+  return GT_OK;
+}
