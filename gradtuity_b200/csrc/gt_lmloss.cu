@@ -413,10 +413,12 @@ Linear linear_layout(gt_ctx* ctx, void* saved, void* scratch, long long M, long 
   if (p.words > V) p.words = V;
   p.pitch_v = (p.words + 7) / 8 * 8;
   l.pieces = (int)((V + p.words - 1) / p.words);
-  // dx has few tiles when there are few rows: its words are then shared out so that every pair of CTAs has about two units
-  const long long tiles = (M + LM_TILE - 1) / LM_TILE * ((E + LM_TILE - 1) / LM_TILE), pairs = ctx->sm_count / 2;
-  const long long most = (p.words + 4 * LM_KBLOCK - 1) / (4 * LM_KBLOCK);
-  long long split = tiles < pairs ? 2 * pairs / tiles : 1;
+  // A dx tile runs over all words of a piece.  Where that is long against what a pair of CTAs has to do in the whole step (few rows:
+  // few tiles, large pieces), its words are shared out, and the shares added up afterwards.
+  const long long tm = (M + LM_TILE - 1) / LM_TILE, te = (E + LM_TILE - 1) / LM_TILE, tv = (p.words + LM_TILE - 1) / LM_TILE;
+  const long long ke = (E + LM_KBLOCK - 1) / LM_KBLOCK, kv = (p.words + LM_KBLOCK - 1) / LM_KBLOCK, km = (M + LM_KBLOCK - 1) / LM_KBLOCK;
+  const long long pairs = ctx->sm_count / 2, step = tm * te * kv + tv * te * km + (l.pieces > 1 ? tm * tv * ke : 0);
+  const long long split = (3 * kv * pairs / 2 + step - 1) / step, most = (kv + 3) / 4;
   p.dx_split = (int)(split < most ? split : most);
 
   LmCarve c = {(char*)saved, 0};

@@ -107,6 +107,7 @@ struct LmRows {
   const float* upstream; int reduction;
   float* dw; int acc_dw;
   float* dx_part;                          // (parts, M, E); null: no dx wanted
+  int cw, c;                               // warps that share the columns, columns a lane
 };
 constexpr long long LM_ROWS_WORK = 64ll << 20;
 bool gt_lm_few_rows(long long M, long long V, long long E);

@@ -2,10 +2,11 @@
 // (and writing dW), and a small problem is launches and latencies; the tensor-core path pays for splitting W into halves first,
 // and for tiles of 256 rows.
 //
-// A block of eight warps takes 32 words at a time.  The E columns are shared out over its lanes, C of them each, and MT rows of x stay
-// in registers; every lane multiplies its columns of a few words with its columns of the rows, the 32 lanes add up by exchanging
-// halves (one exchange per value instead of five), and the warps' sums meet in shared memory.  So W is read once, straight from
-// memory in whole lines, and no operand passes through shared memory.
+// A block of eight warps takes 32 words at a time.  The E columns are shared out over the lanes of CW warps (1, 2, 4 or 8), C columns
+// each, and the words over the 8 / CW groups of such warps; MT rows of x stay in registers.  Every lane multiplies its columns of a
+// few words with its columns of the rows, the 32 lanes add up by exchanging halves (one exchange per value instead of five), and
+// the warps' sums meet in shared memory.  So W is read once, straight from memory in whole lines, and no operand passes through
+// shared memory.  Loads are never guarded: addresses past the end are pulled back, and what comes of them is not used.
 // Forward: running maximum and sum of each row; the last block to end joins the blocks' and, for cross entropy, takes the losses.
 // Backward: the logits again, G = c (p - q), then from the same words dx += G w (in registers, one partial sum per block, added up
 // in the blocks' order by a second kernel) and dW = G^T x, written straight out.
@@ -52,45 +53,68 @@ __device__ __forceinline__ void lanes_sum(float (&v)[N]) {
   }
 }
 
-template <int MT> struct Words { static constexpr int N = MT == 1 ? 16 : MT == 4 ? 8 : 4; };     // words multiplied at a time
+// Words loaded at a time, and multiplied at a time.
+template <int MT, int C> struct Words {
+  static constexpr int SUM = MT == 1 ? 16 : MT == 4 ? 8 : 4;
+  static constexpr int LOAD = MT == 16 && C <= 2 ? 8 : SUM;
+};
 
 struct Rows {
   LmRows r;
   int* status;
 };
 
-// The block's logits of 32 words and MT rows: each warp leaves its columns' share in red[warp][row][word].
+// Where a thread stands: its group of warps, its first column, its group's words among the 32.
+struct Place {
+  int part, group, col0, word0, words;
+};
+template <int C>
+__device__ __forceinline__ Place place_of(int cw) {
+  const int warp = threadIdx.x >> 5;
+  Place p;
+  p.part = warp & (cw - 1);
+  p.group = warp / cw;
+  p.col0 = p.part * 32 * C + (threadIdx.x & 31);
+  p.words = WORDS * cw / WARPS;
+  p.word0 = p.group * p.words;
+  return p;
+}
+
+// The block's logits of 32 words and MT rows: each warp leaves its columns' share in red[part][row][word].
 template <int MT, int C>
-__device__ __forceinline__ void dots(const float (&x)[MT][C], const float* __restrict__ w, long long v0, int V, int E, int col0, float* red) {
-  constexpr int WS = Words<MT>::N;
+__device__ __forceinline__ void dots(const float (&x)[MT][C], const float* __restrict__ w, long long v0, int V, int E, const Place& at, float* red) {
+  constexpr int WS = Words<MT, C>::SUM, WL = Words<MT, C>::LOAD, N = WS * MT;
   const int lane = threadIdx.x & 31;
+  const float* col[C];
 #pragma unroll
-  for (int s = 0; s < WORDS; s += WS) {
-    float b[WS][C];
+  for (int c = 0; c < C; ++c) col[c] = w + min(at.col0 + 32 * c, E - 1);        // x is 0 past the last column
+#pragma unroll 1
+  for (int s = 0; s < at.words; s += WL) {
+    float b[WL][C];
 #pragma unroll
-    for (int i = 0; i < WS; ++i)
+    for (int i = 0; i < WL; ++i) {
+      const long long v = min(v0 + at.word0 + s + i, (long long)V - 1) * E;
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        const int col = col0 + 32 * c;
-        b[i][c] = v0 + s + i < V && col < E ? w[(v0 + s + i) * E + col] : 0.0f;
-      }
-    float a[WS * MT];
+      for (int c = 0; c < C; ++c) b[i][c] = col[c][v];
+    }
 #pragma unroll
-    for (int i = 0; i < WS; ++i)
+    for (int h = 0; h < WL; h += WS) {
+      float a[N];
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        float t = 0.0f;
+      for (int i = 0; i < WS; ++i)
 #pragma unroll
-        for (int c = 0; c < C; ++c) t = fmaf(x[m][c], b[i][c], t);
-        a[i * MT + m] = t;
-      }
-    lanes_sum<WS * MT>(a);
-    constexpr int PER = WS * MT / 32 > 0 ? WS * MT / 32 : 1;
-    if (WS * MT >= 32 || (lane & (32 / (WS * MT > 32 ? 32 : WS * MT) - 1)) == 0) {
+        for (int m = 0; m < MT; ++m) {
+          float t = x[m][0] * b[h + i][0];
 #pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        const int at = WS * MT >= 32 ? lane * PER + j : lane * (WS * MT) / 32;
-        red[(at % MT) * WORDS + s + at / MT] = a[j];
+          for (int c = 1; c < C; ++c) t = fmaf(x[m][c], b[h + i][c], t);
+          a[i * MT + m] = t;
+        }
+      lanes_sum<N>(a);
+#pragma unroll
+      for (int j = 0; j < (N >= 32 ? N / 32 : 1); ++j) {
+        const int k = N >= 32 ? lane * (N / 32) + j : lane * N / 32;             // which sum this lane holds
+        const int word = at.word0 + s + h + k / MT;
+        if (word < WORDS && (N >= 32 || (lane & (32 / (N < 32 ? N : 32) - 1)) == 0)) red[(k % MT) * WORDS + word] = a[j];
       }
     }
   }
@@ -109,18 +133,21 @@ __device__ __forceinline__ void load_rows(float (&x)[MT][C], const float* __rest
   }
 }
 
-// Row t's (m log2 e, s) from the blocks' partial ones, by a warp.
-__device__ __forceinline__ float2 join_parts(const float2* partial, int parts, long long M, long long t) {
+// Row t's (m log2 e, s) from the blocks' partial ones, by `lanes` lanes of a warp that stand together.
+__device__ __forceinline__ float2 join_parts(const float2* partial, int parts, long long M, long long t, int l, int lanes) {
   float m = -INFINITY, s = 0.0f;
-  for (int j = threadIdx.x & 31; j < parts; j += 32) {
+#pragma unroll 4
+  for (int j = l; j < parts; j += lanes) {
     const float2 b = __ldcg(partial + (long long)j * M + t);
     const float top = fmaxf(m, b.x);
     if (top == -INFINITY) { s += b.y; continue; }
     s = s * gt_ex2(m - top) + b.y * gt_ex2(b.x - top);
     m = top;
   }
-  const float top = warp_max(m);
-  s = warp_sum(top == -INFINITY ? s : s * gt_ex2(m - top));
+  float top = m;
+  for (int o = lanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  s = top == -INFINITY ? s : s * gt_ex2(m - top);
+  for (int o = lanes / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   return make_float2(top, s);
 }
 
@@ -130,10 +157,10 @@ __global__ void __launch_bounds__(THREADS) few_rows_forward_kernel(const Rows a)
   __shared__ float red[2][WARPS][MT * WORDS];
   __shared__ int last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int active = (p.E + 32 * C - 1) / (32 * C);             // warps that have columns
-  const int col0 = warp * 32 * C + lane, m0 = blockIdx.y * MT;
+  const Place at = place_of<C>(p.cw);
+  const int m0 = blockIdx.y * MT;
   float x[MT][C];
-  load_rows<MT, C>(x, p.x, m0, p.M, p.E, col0, nullptr);
+  load_rows<MT, C>(x, p.x, m0, p.M, p.E, at.col0, nullptr);
   constexpr int ROWS = (MT + WARPS - 1) / WARPS;                // rows whose maximum and sum a warp keeps
   float m[ROWS], s[ROWS];
 #pragma unroll
@@ -141,14 +168,14 @@ __global__ void __launch_bounds__(THREADS) few_rows_forward_kernel(const Rows a)
   const float l2 = 1.4426950408889634f / p.T;
   int buf = 0;
   for (long long v0 = (long long)blockIdx.x * WORDS; v0 < p.V; v0 += (long long)gridDim.x * WORDS, buf ^= 1) {
-    if (warp < active) dots<MT, C>(x, p.w, v0, p.V, p.E, col0, red[buf][warp]);
+    dots<MT, C>(x, p.w, v0, p.V, p.E, at, red[buf][at.part]);
     __syncthreads();                                            // the other buffer is free: its readers passed this barrier
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
       const int r = warp + i * WARPS;
       if (r < MT) {
         float z = 0.0f;
-        for (int k = 0; k < active; ++k) z += red[buf][k][r * WORDS + lane];
+        for (int k = 0; k < p.cw; ++k) z += red[buf][k][r * WORDS + lane];
         z = v0 + lane < p.V ? z * l2 : -INFINITY;
         const float top = fmaxf(m[i], warp_max(z));
         if (top != -INFINITY) {
@@ -174,30 +201,40 @@ __global__ void __launch_bounds__(THREADS) few_rows_forward_kernel(const Rows a)
   __syncthreads();
   if (!last) return;
   __threadfence();
+  // a row by a warp, or by eight lanes where rows are short: four rows a warp then, with their loads in flight together
+  const int lanes = p.E <= 256 ? 8 : 32, l = lane & (lanes - 1), per_block = THREADS / lanes;
   double total = 0.0;
   int n = 0;
-  for (int t = warp; t < p.M; t += WARPS) {
-    const float f = p.targets[t];
+  for (int t0 = 0; t0 < p.M; t0 += per_block) {
+    const int t = t0 + threadIdx.x / lanes;
+    const bool row = t < p.M;
+    const float f = row ? p.targets[t] : p.ignore;
     const bool in_range = f >= 0.0f && f < (float)p.V, used = f != p.ignore && in_range;
+    const float* xr = p.x + (long long)(used ? t : 0) * p.E;
+    const float* wr = p.w + (long long)(used ? (int)f : 0) * p.E;
+    float z = 0.0f;
+#pragma unroll 8
+    for (int e = l; e < p.E; e += lanes) z = fmaf(xr[e], wr[e], z);
+    const float2 st = join_parts(p.partial, gridDim.x, p.M, row ? t : 0, l, lanes);
+    for (int o = lanes / 2; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+    if (!row || l != 0) continue;
     float loss = 0.0f;
     if (used) {
-      const float2 st = join_parts(p.partial, gridDim.x, p.M, t);
-      const int id = (int)f;
-      float z = 0.0f;
-      for (int e = lane; e < p.E; e += 32) z = fmaf(p.x[(long long)t * p.E + e], p.w[(long long)id * p.E + e], z);
-      z = warp_sum(z);
       loss = logf(st.y) - (z - st.x * 0.6931471805599453f);
-      if (lane == 0) p.s.stats[t] = st;
+      p.s.stats[t] = st;
       total += loss;
       ++n;
     }
-    if (lane == 0) {
-      if (f != p.ignore && !in_range) atomicExch(a.status, GT_ERR_INVALID_ARG);
-      p.s.ids[t] = used ? (int)f : LM_UNUSED;
-      p.s.q[t] = used ? 1.0f : 0.0f;
-      p.s.weight[t] = used ? 1.0f : 0.0f;
-      if (p.row_loss) p.row_loss[t] = loss;
-    }
+    if (f != p.ignore && !in_range) atomicExch(a.status, GT_ERR_INVALID_ARG);
+    p.s.ids[t] = used ? (int)f : LM_UNUSED;
+    p.s.q[t] = used ? 1.0f : 0.0f;
+    p.s.weight[t] = used ? 1.0f : 0.0f;
+    if (p.row_loss) p.row_loss[t] = loss;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+    n += __shfl_xor_sync(0xffffffffu, n, o);
   }
   __shared__ double totals[WARPS];
   __shared__ int counts[WARPS];
@@ -213,16 +250,17 @@ __global__ void __launch_bounds__(THREADS) few_rows_forward_kernel(const Rows a)
 template <int MT, int C>
 __global__ void __launch_bounds__(THREADS) few_rows_backward_kernel(const Rows a) {
   const LmRows& p = a.r;
-  __shared__ float red[WARPS][MT * WORDS];
+  // the warps' shares of the logits; at the end, dx of half the groups of warps (4 x 32 columns a lane a warp, 4 warps)
+  __shared__ float pool[MT * 512 > WARPS * MT * WORDS ? MT * 512 : WARPS * MT * WORDS];
+  float (*const red)[MT * WORDS] = reinterpret_cast<float (*)[MT * WORDS]>(pool);
   __shared__ __align__(16) float gs[WORDS * MT];                // G, word by word
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int active = (p.E + 32 * C - 1) / (32 * C);
-  const int col0 = warp * 32 * C + lane;
+  const Place at = place_of<C>(p.cw);
   const float l2 = 1.4426950408889634f / p.T;
   constexpr int ROWS = (MT + WARPS - 1) / WARPS;
   for (int m0 = 0; m0 < p.M; m0 += MT) {
     float x[MT][C], dx[MT][C];
-    load_rows<MT, C>(x, p.x, m0, p.M, p.E, col0, p.s.weight);
+    load_rows<MT, C>(x, p.x, m0, p.M, p.E, at.col0, p.s.weight);
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -241,14 +279,14 @@ __global__ void __launch_bounds__(THREADS) few_rows_backward_kernel(const Rows a
       }
     }
     for (long long v0 = (long long)blockIdx.x * WORDS; v0 < p.V; v0 += (long long)gridDim.x * WORDS) {
-      if (warp < active) dots<MT, C>(x, p.w, v0, p.V, p.E, col0, red[warp]);
+      dots<MT, C>(x, p.w, v0, p.V, p.E, at, red[at.part]);
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < ROWS; ++i) {
         const int r = warp + i * WARPS;
         if (r < MT) {
           float z = 0.0f;
-          for (int k = 0; k < active; ++k) z += red[k][r * WORDS + lane];
+          for (int k = 0; k < p.cw; ++k) z += red[k][r * WORDS + lane];
           const int t = m0 + r, v = (int)v0 + lane;
           float g = 0.0f;
           if (t < p.M && p.s.weight[t] != 0.0f && v < p.V) {
@@ -262,46 +300,80 @@ __global__ void __launch_bounds__(THREADS) few_rows_backward_kernel(const Rows a
         }
       }
       __syncthreads();
-      if (warp < active) {
-#pragma unroll 4
-        for (int i = 0; i < WORDS; ++i) {
-          float g[MT];
-          if (MT >= 4) {
+      const int words = min(at.words, (int)min((long long)WORDS, p.V - v0) - at.word0);
+      const bool add = p.acc_dw || m0 > 0;
+      constexpr int GROUP = 4;                                  // words whose loads go out together, ahead of the stores
+#pragma unroll 1
+      for (int i0 = 0; i0 < words; i0 += GROUP) {
+        float b[GROUP][C], d[GROUP][C];
 #pragma unroll
-            for (int m = 0; m < MT; m += 4) *reinterpret_cast<float4*>(g + m) = *reinterpret_cast<const float4*>(gs + i * MT + m);
-          } else {
-            g[0] = gs[i];
-          }
-          const long long v = v0 + i;
-          if (v >= p.V) break;
+        for (int i = 0; i < GROUP; ++i) {
+          const long long row = (v0 + at.word0 + min(i0 + i, words - 1)) * p.E;
 #pragma unroll
           for (int c = 0; c < C; ++c) {
-            const int col = col0 + 32 * c;
-            if (col >= p.E) continue;
-            if (p.dx_part) {
-              const float b = p.w[v * p.E + col];               // read a moment ago: in L1
-#pragma unroll
-              for (int m = 0; m < MT; ++m) dx[m][c] = fmaf(g[m], b, dx[m][c]);
-            }
-            if (p.dw) {
-              float d = p.acc_dw || m0 > 0 ? p.dw[v * p.E + col] : 0.0f;
-#pragma unroll
-              for (int m = 0; m < MT; ++m) d = fmaf(g[m], x[m][c], d);
-              p.dw[v * p.E + col] = d;
-            }
+            const int col = min(at.col0 + 32 * c, p.E - 1);
+            b[i][c] = p.dx_part ? __ldg(p.w + row + col) : 0.0f;        // read a moment ago: in L1
+            d[i][c] = add && p.dw ? p.dw[row + col] : 0.0f;
           }
+        }
+#pragma unroll
+        for (int i = 0; i < GROUP; ++i) {
+          if (i0 + i >= words) break;
+          const float* gi = gs + (at.word0 + i0 + i) * MT;
+#pragma unroll
+          for (int m = 0; m < MT; m += MT >= 4 ? 4 : 1) {
+            float g[4];
+            if (MT >= 4) *reinterpret_cast<float4*>(g) = *reinterpret_cast<const float4*>(gi + m);
+            else g[0] = gi[m];
+#pragma unroll
+            for (int k = 0; k < (MT >= 4 ? 4 : 1); ++k)
+#pragma unroll
+              for (int c = 0; c < C; ++c) {
+                dx[m + k][c] = fmaf(g[k], b[i][c], dx[m + k][c]);
+                d[i][c] = fmaf(g[k], x[m + k][c], d[i][c]);
+              }
+          }
+        }
+        if (p.dw) {
+#pragma unroll
+          for (int i = 0; i < GROUP; ++i)
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+              if (i0 + i < words && at.col0 + 32 * c < p.E) p.dw[(v0 + at.word0 + i0 + i) * p.E + at.col0 + 32 * c] = d[i][c];
         }
       }
       // gs is written again behind the next block's first barrier; red behind this block's second one
     }
-    if (p.dx_part && warp < active) {
+    if (p.dx_part) {
+      // the groups' sums, halving their number each time: the order is the same every time
+      const int cols = p.cw * 32 * C, mine = at.part * 32 * C + lane;
+      for (int half = WARPS / p.cw / 2; half > 0; half >>= 1) {
+        __syncthreads();
+        if (at.group >= half && at.group < 2 * half) {
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+          for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-          const int col = col0 + 32 * c;
-          if (m0 + m < p.M && col < p.E) p.dx_part[((long long)blockIdx.x * p.M + m0 + m) * p.E + col] = dx[m][c];
+            for (int c = 0; c < C; ++c) pool[((at.group - half) * MT + m) * cols + mine + 32 * c] = dx[m][c];
         }
+        __syncthreads();
+        if (at.group < half) {
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int c = 0; c < C; ++c) dx[m][c] += pool[(at.group * MT + m) * cols + mine + 32 * c];
+        }
+      }
+      if (at.group == 0) {
+        float* to = p.dx_part + ((long long)blockIdx.x * p.M + m0) * p.E;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int c = 0; c < C; ++c) {
+            const int col = at.col0 + 32 * c;
+            if (m0 + m < p.M && col < p.E) to[(long long)m * p.E + col] = dx[m][c];
+          }
+      }
+      __syncthreads();
     }
   }
 }
@@ -336,7 +408,7 @@ int launch_as(gt_ctx* ctx, const Rows& a, bool backward) {
 }
 template <int MT>
 int launch_for(gt_ctx* ctx, const Rows& a, bool backward) {
-  switch ((a.r.E + 255) / 256) {
+  switch (a.r.c) {
     case 1: return launch_as<MT, 1>(ctx, a, backward);
     case 2: return launch_as<MT, 2>(ctx, a, backward);
     case 3: return launch_as<MT, 3>(ctx, a, backward);
@@ -344,7 +416,11 @@ int launch_for(gt_ctx* ctx, const Rows& a, bool backward) {
   }
 }
 int launch(gt_ctx* ctx, const LmRows& p, bool backward) {
-  const Rows a = {p, ctx->d_status};
+  Rows a = {p, ctx->d_status};
+  // As many columns a lane as there are, up to four: adding up over lanes and warps costs the same for one column as for four.
+  const int wide = (p.E + 127) / 128;
+  a.r.cw = wide <= 1 ? 1 : wide <= 2 ? 2 : wide <= 4 ? 4 : 8;
+  a.r.c = (p.E + 32 * a.r.cw - 1) / (32 * a.r.cw);
   if (p.M == 1) return launch_for<1>(ctx, a, backward);
   if (p.M <= 4) return launch_for<4>(ctx, a, backward);
   return launch_for<16>(ctx, a, backward);
