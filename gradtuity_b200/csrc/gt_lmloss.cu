@@ -37,21 +37,49 @@ __device__ __forceinline__ float warp_max(float v) {
 
 // ---- targets -------------------------------------------------------------------------------------
 
-// Cross entropy: one target of q = 1 per row.  An id outside the vocabulary sets the status word.
-__global__ void __launch_bounds__(256) hard_targets_kernel(const float* __restrict__ targets, long long M, long long V, float ignore,
-                                                           LmSaved s, float* __restrict__ row_loss, int* status) {
-  const long long t = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  bool used = false;
-  if (t < M) {
-    const float f = targets[t];
-    const bool in_range = f >= 0.0f && f < (float)V;
-    used = f != ignore && in_range;
-    if (f != ignore && !in_range) atomicExch(status, GT_ERR_INVALID_ARG);
-    s.ids[t] = used ? (int)f : LM_UNUSED;
-    s.q[t] = used ? 1.0f : 0.0f;
-    s.weight[t] = used ? 1.0f : 0.0f;
-    s.konst[t] = 0.0f;
-    if (!used) row_loss[t] = 0.0f;
+// Rows that count, in order, a block of 1024 threads at a time: `counts` is this thread's row t.  base: rows before.
+__device__ __forceinline__ void append_rows(bool counts, long long t, int& base, int* row_of) {
+  __shared__ int sums[32];
+  const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
+  const unsigned mask = __ballot_sync(0xffffffffu, counts);
+  if (l == 0) sums[w] = __popc(mask);
+  __syncthreads();
+  const int mine = sums[l];
+  int before = w > l ? mine : 0, all = mine;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+  }
+  if (counts) row_of[base + before + __popc(mask & ((1u << l) - 1))] = (int)t;
+  base += all;
+  __syncthreads();
+}
+
+// Cross entropy: one target of q = 1 per row, and the rows that count.  An id outside the vocabulary sets the status word.  One block,
+// which also clears what later kernels count in.
+__global__ void __launch_bounds__(1024) hard_targets_kernel(const float* __restrict__ targets, long long M, long long V, float ignore, LmSaved s,
+                                                            float* __restrict__ row_loss, int* counters, int* status) {
+  int base = 0;
+  for (long long t0 = 0; t0 < M; t0 += 1024) {
+    const long long t = t0 + threadIdx.x;
+    bool used = false;
+    if (t < M) {
+      const float f = targets[t];
+      const bool in_range = f >= 0.0f && f < (float)V;
+      used = f != ignore && in_range;
+      if (f != ignore && !in_range) atomicExch(status, GT_ERR_INVALID_ARG);
+      s.ids[t] = used ? (int)f : LM_UNUSED;
+      s.q[t] = used ? 1.0f : 0.0f;
+      s.weight[t] = used ? 1.0f : 0.0f;
+      s.konst[t] = 0.0f;
+      if (!used) row_loss[t] = 0.0f;
+    }
+    append_rows(used, t, base, s.row_of);
+  }
+  if (threadIdx.x == 0) {
+    *counters = 0;
+    s.scalars->count = base; s.scalars->done = 0; s.scalars->amax_x = 0; s.scalars->amax_w = 0;
   }
 }
 
@@ -112,29 +140,14 @@ __global__ void __launch_bounds__(128) top_targets_kernel(const float* __restric
   }
 }
 
-// row_of: the rows that count, in order; count: how many.  One block.
-__global__ void __launch_bounds__(1024) compact_rows_kernel(long long M, LmSaved s) {
-  __shared__ int sums[32];
-  const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
+// The same for a distillation's rows, whose targets are there.
+__global__ void __launch_bounds__(1024) compact_rows_kernel(long long M, LmSaved s, int* counters) {
   int base = 0;
   for (long long t0 = 0; t0 < M; t0 += 1024) {
     const long long t = t0 + threadIdx.x;
-    const bool counts = t < M && s.weight[t] != 0.0f;
-    const unsigned mask = __ballot_sync(0xffffffffu, counts);
-    if (l == 0) sums[w] = __popc(mask);
-    __syncthreads();
-    const int mine = sums[l];
-    int before = w > l ? mine : 0, all = mine;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      before += __shfl_xor_sync(0xffffffffu, before, o);
-      all += __shfl_xor_sync(0xffffffffu, all, o);
-    }
-    if (counts) s.row_of[base + before + __popc(mask & ((1u << l) - 1))] = (int)t;
-    base += all;
-    __syncthreads();
+    append_rows(t < M && s.weight[t] != 0.0f, t, base, s.row_of);
   }
-  if (threadIdx.x == 0) s.scalars->count = base;
+  if (threadIdx.x == 0) { *counters = 0; s.scalars->count = base; }
 }
 
 // ---- operands of the linear forms: largest value, then the split into halves ------------------------
@@ -146,7 +159,7 @@ __global__ void __launch_bounds__(256) largest_kernel(const float* __restrict__ 
   const long long rows = is_x ? s.scalars->count : V;
   const int first = is_x ? blockIdx.x : blockIdx.x - blocks_x, step = is_x ? blocks_x : gridDim.x - blocks_x;
   const float* src = is_x ? x : w;
-  const bool vec = ((uintptr_t)src & 15) == 0 && E % 4 == 0;
+  const bool vec = ((uintptr_t)src & 15) == 0;
   unsigned m = 0;
   auto see = [&](float f) {
     const unsigned b = __float_as_uint(f) & 0x7fffffffu;
@@ -164,6 +177,7 @@ __global__ void __launch_bounds__(256) largest_kernel(const float* __restrict__ 
       for (int k = 0; k < 4; ++k) { see(a[k].x); see(a[k].y); see(a[k].z); see(a[k].w); }
     }
     for (; i < n; i += (long long)step * 256) { const float4 a = p[i]; see(a.x); see(a.y); see(a.z); see(a.w); }
+    if (first == 0 && threadIdx.x < (int)(rows * E - 4 * n)) see(src[4 * n + threadIdx.x]);
   } else {
     for (long long r = (long long)first * 8 + (threadIdx.x >> 5); r < rows; r += (long long)step * 8) {
       const float* p = src + (is_x ? s.row_of[r] : r) * E;
@@ -231,9 +245,9 @@ __global__ void __launch_bounds__(256) split_kernel(const float* __restrict__ x,
 // ---- rows ------------------------------------------------------------------------------------------
 
 // The linear forms: (m, s) of the rows that count from the parts' (tiles of words, or blocks).  32 rows a block, their parts shared
-// out over the warps, so that a warp reads whole lines.  by_row: parts and stats go by row, not by compact row.
-__global__ void __launch_bounds__(256) join_stats_kernel(const float2* __restrict__ partial, int parts, long long M, int by_row, LmSaved s) {
-  __shared__ float2 red[8][32];
+// out over 32 warps, so that a warp reads whole lines.  by_row: parts and stats go by row, not by compact row.
+__global__ void __launch_bounds__(1024) join_stats_kernel(const float2* __restrict__ partial, int parts, long long M, int by_row, LmSaved s) {
+  __shared__ float2 red[32][33];
   const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
   const long long i = (long long)blockIdx.x * 32 + l;
   const bool live = i < s.scalars->count;
@@ -247,13 +261,16 @@ __global__ void __launch_bounds__(256) join_stats_kernel(const float2* __restric
   };
   if (live) {
 #pragma unroll 4
-    for (int j = w; j < parts; j += 8) add(partial[(long long)j * M + at]);
+    for (int j = w; j < parts; j += 32) add(partial[(long long)j * M + at]);
   }
   red[w][l] = make_float2(m, sum);
   __syncthreads();
-  if (w != 0 || !live) return;
-  for (int k = 1; k < 8; ++k) add(red[k][l]);
-  s.stats[at] = make_float2(m, sum);
+  // warp w joins row w's 32 shares, in an order that is the same every time
+  const float2 mine = red[l][w];
+  const float top = warp_max(mine.x);
+  sum = warp_sum(top == -INFINITY ? mine.y : mine.y * gt_ex2(mine.x - top));
+  const long long r = (long long)blockIdx.x * 32 + w;
+  if (l == 0 && r < s.scalars->count) s.stats[by_row ? s.row_of[r] : r] = make_float2(top, sum);
 }
 
 // Losses of the compact rows, from the logits of their targets, taken in 32 bits straight from x and w.  WARPS_A_ROW warps share a
@@ -323,11 +340,20 @@ __global__ void __launch_bounds__(256) target_loss_kernel(float* __restrict__ ro
   }
 }
 
-// What the rows' gradients are multiplied by.  The halves of G hold 2^14 u (p - q), u = 1, or with a gradient per row that row's
-// share of a power of two P above the largest; the rest goes into the products' own factors.  One block.
-__global__ void __launch_bounds__(1024) grad_factor_kernel(const float* __restrict__ upstream, int reduction, float T, LmSaved s) {
+// Before the backward walk.  Block 0: what the rows' gradients are multiplied by.  The halves of G hold 2^14 u (p - q), u = 1, or with
+// a gradient per row that row's share of a power of two P above the largest; the rest goes into the products' own factors.  It
+// also clears the steps' counters.  The other blocks (if any): zeros for dx of the rows that do not count, a warp per row.
+__global__ void __launch_bounds__(1024) begin_backward_kernel(const float* __restrict__ upstream, int reduction, float T, LmSaved s, int* counters,
+                                                              int steps, float* __restrict__ dx, long long M, long long E) {
+  if (blockIdx.x > 0) {
+    for (long long t = (long long)(blockIdx.x - 1) * 32 + (threadIdx.x >> 5); t < M; t += (long long)(gridDim.x - 1) * 32)
+      if (s.weight[t] == 0.0f)
+        for (long long e = threadIdx.x & 31; e < E; e += 32) dx[t * E + e] = 0.0f;
+    return;
+  }
   __shared__ unsigned part[32];
   const int n = s.scalars->count;
+  for (int i = threadIdx.x; i < steps; i += 1024) counters[i] = 0;
   float P = 1.0f;
   if (reduction == GT_REDUCE_NONE) {
     unsigned m = 0;
@@ -352,13 +378,6 @@ __global__ void __launch_bounds__(1024) grad_factor_kernel(const float* __restri
     s.scalars->dx = ldexpf(c, scale_exponent(s.scalars->amax_w) - 14);
     s.scalars->dw = ldexpf(c, scale_exponent(s.scalars->amax_x) - 14);
   }
-}
-
-// dx of rows that do not count.  A block per row.
-__global__ void __launch_bounds__(128) zero_rows_kernel(float* __restrict__ dx, long long E, LmSaved s) {
-  const long long t = blockIdx.x;
-  if (s.weight[t] != 0.0f) return;
-  for (long long e = threadIdx.x; e < E; e += 128) dx[t * E + e] = 0.0f;
 }
 
 // dx (+)= the shares of a piece, in order.
@@ -398,6 +417,7 @@ Linear linear_layout(gt_ctx* ctx, void* saved, void* scratch, long long M, long 
     LmCarve c = {(char*)saved, 0}, f = {(char*)scratch, 0};
     l.s = lm_saved(c, M, K);
     l.saved_bytes = c.at;
+    p.counters = f.take<int>(1);
     LmCarve b = f;
     l.row_loss = f.take<float>(M);
     p.partial = f.take<float2>((size_t)gt_lm_rows_parts(ctx, M, V, false) * M);
@@ -451,17 +471,15 @@ LmRows rows_problem(const Linear& l, const float* x, const float* w, long long M
   return r;
 }
 
-int prepare_linear(gt_ctx* ctx, const LmSaved& s, float* row_loss, const float* targets, float ignore, const float* ids, const float* teacher,
-                    long long M, long long V, long long K, float T) {
+int prepare_linear(gt_ctx* ctx, const LmSaved& s, int* counters, float* row_loss, const float* targets, float ignore, const float* ids,
+                   const float* teacher, long long M, long long V, long long K, float T) {
   if (targets) {
-    GT_CUDA_OK(ctx, cudaMemsetAsync(s.scalars, 0, sizeof(LmScalars), ctx->stream));
-    hard_targets_kernel<<<(unsigned)((M + 255) / 256), 256, 0, ctx->stream>>>(targets, M, V, ignore, s, row_loss, ctx->d_status);
-    ctx->launches += 1;
+    hard_targets_kernel<<<1, 1024, 0, ctx->stream>>>(targets, M, V, ignore, s, row_loss, counters, ctx->d_status);
   } else {
     int rc = gt_lm_top_targets(ctx, s, row_loss, ids, teacher, M, V, K, T);
     if (rc != GT_OK) return rc;
+    compact_rows_kernel<<<1, 1024, 0, ctx->stream>>>(M, s, counters);
   }
-  compact_rows_kernel<<<1, 1024, 0, ctx->stream>>>(M, s);
   GT_CUDA_OK(ctx, cudaGetLastError());
   ctx->launches += 1;
   return GT_OK;
@@ -471,7 +489,7 @@ int finish_rows(gt_ctx* ctx, float* row_loss, float* loss, const float2* partial
                 long long E, long long K, float T, int reduction, int by_row, const LmSaved& s) {
   float* out = reduction == GT_REDUCE_NONE ? nullptr : loss;
   const int mean = reduction == GT_REDUCE_MEAN;
-  join_stats_kernel<<<(unsigned)((M + 31) / 32), 256, 0, ctx->stream>>>(partial, parts, M, by_row, s);
+  join_stats_kernel<<<(unsigned)((M + 31) / 32), 1024, 0, ctx->stream>>>(partial, parts, M, by_row, s);
   if (K == 1) target_loss_kernel<1><<<(unsigned)((M + 7) / 8), 256, 0, ctx->stream>>>(row_loss, out, x, w, M, (int)E, (int)K, T, mean, by_row, s);
   else target_loss_kernel<8><<<(unsigned)M, 256, 0, ctx->stream>>>(row_loss, out, x, w, M, (int)E, (int)K, T, mean, by_row, s);
   GT_CUDA_OK(ctx, cudaGetLastError());
@@ -488,7 +506,7 @@ int linear_forward(gt_ctx* ctx, float* loss, void* saved, void* scratch, const f
     LmRows r = rows_problem(l, x, w, M, V, E, K, T, reduction);
     r.parts = gt_lm_rows_parts(ctx, M, V, false);
     if (!targets) {
-      int rc = prepare_linear(ctx, s, rows, nullptr, 0.0f, ids, teacher, M, V, K, T);
+      int rc = prepare_linear(ctx, s, l.p.counters, rows, nullptr, 0.0f, ids, teacher, M, V, K, T);
       if (rc == GT_OK) rc = gt_lm_rows_forward(ctx, r);
       return rc != GT_OK ? rc : finish_rows(ctx, rows, loss, l.p.partial, r.parts, x, w, M, E, K, T, reduction, 1, s);
     }
@@ -498,9 +516,8 @@ int linear_forward(gt_ctx* ctx, float* loss, void* saved, void* scratch, const f
     r.loss = reduction == GT_REDUCE_NONE ? nullptr : loss;
     return gt_lm_rows_forward(ctx, r);
   }
-  int rc = prepare_linear(ctx, s, rows, targets, ignore, ids, teacher, M, V, K, T);
+  int rc = prepare_linear(ctx, s, l.p.counters, rows, targets, ignore, ids, teacher, M, V, K, T);
   if (rc != GT_OK) return rc;
-  GT_CUDA_OK(ctx, cudaMemsetAsync(l.p.counters, 0, sizeof(int), ctx->stream));
   const long long most = 8ll * ctx->sm_count;
   auto blocks = [&](long long n) { return (int)((n + 7) / 8 < most ? (n + 7) / 8 : most); };
   const int bx = blocks(M), bw = blocks(V);
@@ -563,15 +580,10 @@ extern "C" int gt_linear_loss_backward(gt_ctx* ctx, float* dx, float* dw, void* 
   }
   LmProblem& p = l.p;
   p.dx = dx; p.dw = dw; p.acc_dx = acc_dx; p.acc_dw = acc_dw;
-  GT_CUDA_OK(ctx, cudaMemsetAsync(p.counters, 0, sizeof(int) * (l.pieces + 1), ctx->stream));
-  grad_factor_kernel<<<1, 1024, 0, ctx->stream>>>(upstream, reduction, temperature, l.s);
+  const long long zero_blocks = dx && !acc_dx ? ((M + 31) / 32 < ctx->sm_count ? (M + 31) / 32 : ctx->sm_count) : 0;
+  begin_backward_kernel<<<(unsigned)(1 + zero_blocks), 1024, 0, ctx->stream>>>(upstream, reduction, temperature, l.s, p.counters, l.pieces + 1, dx, M, E);
   GT_CUDA_OK(ctx, cudaGetLastError());
   ctx->launches += 1;
-  if (dx && !acc_dx) {
-    zero_rows_kernel<<<(unsigned)M, 128, 0, ctx->stream>>>(dx, E, l.s);
-    GT_CUDA_OK(ctx, cudaGetLastError());
-    ctx->launches += 1;
-  }
   for (int piece = 0; piece <= l.pieces; ++piece) {
     int rc = gt_lm_step(ctx, p, piece);
     if (rc != GT_OK) return rc;

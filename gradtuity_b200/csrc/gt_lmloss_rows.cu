@@ -378,23 +378,22 @@ __global__ void __launch_bounds__(THREADS) few_rows_backward_kernel(const Rows a
   }
 }
 
-// dx (+)= the blocks' shares in their order: 32 columns of a row per block, the warps take every eighth share.
-__global__ void __launch_bounds__(THREADS) few_rows_dx_kernel(float* __restrict__ dx, const float* __restrict__ part, int parts, long long M, int E, int add) {
-  __shared__ float sums[WARPS][32];
+// dx (+)= the blocks' shares: 32 columns of a row per block, a warp takes every 32nd share, and the warps are added in order.
+__global__ void __launch_bounds__(1024) few_rows_dx_kernel(float* __restrict__ dx, const float* __restrict__ part, int parts, long long M, int E, int add) {
+  __shared__ float sums[32][33];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int col = blockIdx.x * 32 + lane;
   const long long t = blockIdx.y;
   float s = 0.0f;
   if (col < E) {
 #pragma unroll 8
-    for (int j = warp; j < parts; j += WARPS) s += part[((long long)j * M + t) * E + col];
+    for (int j = warp; j < parts; j += 32) s += part[((long long)j * M + t) * E + col];
   }
   sums[warp][lane] = s;
   __syncthreads();
-  if (warp == 0 && col < E) {
-    for (int k = 1; k < WARPS; ++k) s += sums[k][lane];
-    dx[t * E + col] = add ? dx[t * E + col] + s : s;
-  }
+  s = warp_sum(sums[lane][warp]);                               // the 32 warps' sums of column `warp`
+  const int mine = blockIdx.x * 32 + warp;
+  if (lane == 0 && mine < E) dx[t * E + mine] = add ? dx[t * E + mine] + s : s;
 }
 
 template <int MT, int C>
@@ -435,7 +434,7 @@ bool gt_lm_few_rows(long long M, long long V, long long E) {
 
 int gt_lm_rows_parts(gt_ctx* ctx, long long M, long long V, bool backward) {
   const long long blocks = (V + WORDS - 1) / WORDS, tiles = M <= 16 ? 1 : (M + 15) / 16;
-  long long most = 2ll * ctx->sm_count;                          // two blocks an SM
+  long long most = (M <= 1 ? 3ll : 2ll) * ctx->sm_count;         // blocks an SM; one row: 138 us with two, 130 with three, 137 with four
   if (!backward) most = (most + tiles - 1) / tiles;
   return (int)(blocks < most ? blocks : most);
 }
@@ -445,7 +444,7 @@ int gt_lm_rows_forward(gt_ctx* ctx, const LmRows& p) { return launch(ctx, p, fal
 int gt_lm_rows_backward(gt_ctx* ctx, const LmRows& p, float* dx, int acc_dx) {
   int rc = launch(ctx, p, true);
   if (rc != GT_OK || !dx) return rc;
-  few_rows_dx_kernel<<<dim3((unsigned)((p.E + 31) / 32), (unsigned)p.M), THREADS, 0, ctx->stream>>>(dx, p.dx_part, p.parts, p.M, p.E, acc_dx);
+  few_rows_dx_kernel<<<dim3((unsigned)((p.E + 31) / 32), (unsigned)p.M), 1024, 0, ctx->stream>>>(dx, p.dx_part, p.parts, p.M, p.E, acc_dx);
   GT_CUDA_OK(ctx, cudaGetLastError());
   ctx->launches += 1;
   return GT_OK;

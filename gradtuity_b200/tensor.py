@@ -23,6 +23,7 @@ import os
 import struct
 from contextlib import contextmanager
 from ctypes import byref, c_size_t, c_void_p
+from functools import lru_cache
 from typing import Callable, Optional
 
 from . import _lib
@@ -146,6 +147,21 @@ class _GradGroup:
             cuda_memset(ptr, 0, self.numel_each * F32)
         self.written[index] = True
         return Tensor._from_ptr(ptr, shape, owns_memory=False, base=self.storage)
+
+
+@lru_cache(maxsize=256)
+def _linear_loss_sizes(M: int, V: int, E: int, top: int, precision: int) -> tuple[int, int]:
+    """Bytes that a linear loss keeps for its backward pass, and of its scratch memory."""
+    saved, scratch = c_size_t(0), c_size_t(0)
+    _call("gt_linear_loss_sizes", M, V, E, top, precision, byref(saved), byref(scratch))
+    return saved.value, scratch.value
+
+
+@lru_cache(maxsize=256)
+def _topk_distillation_size(rows: int, classes: int, top: int) -> int:
+    saved = c_size_t(0)
+    _call("gt_topk_distillation_sizes", rows, classes, top, byref(saved))
+    return saved.value
 
 
 def ensure_grad(t: "Tensor") -> None:
@@ -1214,21 +1230,26 @@ class Tensor:
         prec = _gemm.precision_of(precision)
         M, E = self._shape
         V, _ = weight._shape
-        n_saved, n_scratch = c_size_t(0), c_size_t(0)
-        _call("gt_linear_loss_sizes", M, V, E, top, prec, byref(n_saved), byref(n_scratch))
-        saved = alloc_storage(n_saved.value)
+        n_saved, n_scratch = _linear_loss_sizes(M, V, E, top, prec)
+        # small scratch memory stays with what is saved for the backward pass, which uses it again
+        keep = n_scratch <= (4 << 20)
+        saved = alloc_storage(n_saved + n_scratch if keep else n_saved)
+        work = saved.ptr + n_saved if keep else 0
+        x, x_ptr, w_ptr = self, self.ptr, weight.ptr
         out = empty_tensor((M,) if reduction == _lib.REDUCTIONS["none"] else (1,))
-        with temp_storage(n_scratch.value) as scratch:
-            _call(entry, _vp(out.ptr), _vp(saved.ptr), _vp(scratch.ptr), _vp(self.ptr), _vp(weight.ptr), *(_vp(t.ptr) for t in given), M, V, E,
-                  *extra, reduction, prec)
-        x = self
+        scratch = None if keep else alloc_storage(n_scratch)
+        _call(entry, out.ptr, saved.ptr, work or scratch.ptr, x_ptr, w_ptr, *(t.ptr for t in given), M, V, E, *extra, reduction, prec)
+        if scratch is not None:
+            scratch.free()
 
         def _backward(g: "Tensor") -> None:
-            dx, acc_dx = grad_target(x) if x.requires_grad else (0, False)
-            dw, acc_dw = grad_target(weight) if weight.requires_grad else (0, False)
-            with temp_storage(n_scratch.value) as scratch:
-                _call("gt_linear_loss_backward", _vp(dx), _vp(dw), _vp(saved.ptr), _vp(scratch.ptr), _vp(x.ptr), _vp(weight.ptr), _vp(g.ptr),
-                      M, V, E, top, temperature, reduction, prec, int(acc_dx), int(acc_dw))
+            dx, acc_dx = grad_target(x) if x.requires_grad else (None, False)
+            dw, acc_dw = grad_target(weight) if weight.requires_grad else (None, False)
+            scratch = None if keep else alloc_storage(n_scratch)
+            _call("gt_linear_loss_backward", dx, dw, saved.ptr, work or scratch.ptr, x.ptr, weight.ptr, g.ptr, M, V, E, top, temperature, reduction,
+                  prec, acc_dx, acc_dw)
+            if scratch is not None:
+                scratch.free()
 
         out._set_graph(parents=(self, weight), backward_fn=_backward)
         return out
@@ -1270,9 +1291,7 @@ class Tensor:
             raise ValueError(f"topk_distillation expects 2D logits, got ndim={self.ndim}")
         Bn, C = self._shape
         top = self._teacher_checks("topk_distillation", Bn, teacher_ids, teacher_logits)
-        n_saved = c_size_t(0)
-        _call("gt_topk_distillation_sizes", Bn, C, top, byref(n_saved))
-        saved = alloc_storage(n_saved.value)
+        saved = alloc_storage(_topk_distillation_size(Bn, C, top))
         out = empty_tensor((Bn,) if reduction == "none" else (1,))
         x_ptr, x_ld = self._rows()
         T = float(temperature)
@@ -1280,8 +1299,7 @@ class Tensor:
         # launch, for the upstream gradient of 1 that backward() seeds; another upstream gradient rescales it.
         early = empty_padded_tensor(self.shape, x_ld) if self.requires_grad and self.grad is None and reduction != "none" else None
         e_ptr, e_ld = early._rows() if early is not None else (0, 0)
-        _call("gt_topk_distillation", _vp(out.ptr), _vp(saved.ptr), _vp(e_ptr), e_ld, _vp(x_ptr), x_ld, _vp(teacher_ids.ptr), _vp(teacher_logits.ptr),
-              Bn, C, top, T, mode)
+        _call("gt_topk_distillation", out.ptr, saved.ptr, e_ptr or None, e_ld, x_ptr, x_ld, teacher_ids.ptr, teacher_logits.ptr, Bn, C, top, T, mode)
         logits = self
 
         def _backward(g: "Tensor") -> None:
@@ -1301,7 +1319,7 @@ class Tensor:
                 logits.grad = empty_padded_tensor(logits.shape, logits._rows()[1])
             d_ptr, d_ld = logits.grad._rows()
             lx_ptr, lx_ld = logits._rows()
-            _call("gt_topk_distillation_backward", _vp(d_ptr), d_ld, _vp(saved.ptr), _vp(lx_ptr), lx_ld, _vp(g.ptr), Bn, C, top, T, mode, 0 if fresh else 1)
+            _call("gt_topk_distillation_backward", d_ptr, d_ld, saved.ptr, lx_ptr, lx_ld, g.ptr, Bn, C, top, T, mode, not fresh)
 
         out._set_graph(parents=(self,), backward_fn=_backward)
         return out
