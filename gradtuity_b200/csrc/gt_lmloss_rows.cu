@@ -2,7 +2,7 @@
 // (and writing dW), and a small problem is launches and latencies; the tensor-core path pays for splitting W into halves first,
 // and for tiles of 256 rows.
 //
-// A block of eight warps takes 32 words at a time.  The E columns are shared out over the lanes of CW warps (1, 2, 4 or 8), C columns
+// A block of eight warps takes 32 words at a time (one row: 16).  The E columns are shared out over the lanes of CW warps (1, 2, 4 or 8), C columns
 // each, and the words over the 8 / CW groups of such warps; MT rows of x stay in registers.  Every lane multiplies its columns of a
 // few words with its columns of the rows, the 32 lanes add up by exchanging halves (one exchange per value instead of five), and
 // the warps' sums meet in shared memory.  So W is read once, straight from memory in whole lines, and no operand passes through
@@ -16,7 +16,7 @@
 
 namespace {
 
-constexpr int THREADS = 256, WARPS = 8, WORDS = 32;
+constexpr int THREADS = 256, WARPS = 8;
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -57,6 +57,9 @@ __device__ __forceinline__ void lanes_sum(float (&v)[N]) {
 template <int MT, int C> struct Words {
   static constexpr int SUM = MT == 1 ? 16 : MT == 4 ? 8 : 4;
   static constexpr int LOAD = MT == 16 && C <= 2 ? 8 : SUM;
+  // A block's words.  One row: few enough for a warp to keep them in registers between the two uses that the backward pass has of them.
+  static constexpr int BLOCK = MT == 1 ? 16 : 32;
+  static constexpr bool KEPT = BLOCK == LOAD;
 };
 
 struct Rows {
@@ -64,33 +67,33 @@ struct Rows {
   int* status;
 };
 
-// Where a thread stands: its group of warps, its first column, its group's words among the 32.
+// Where a thread stands: its group of warps, its first column, its group's words among the block's.
 struct Place {
   int part, group, col0, word0, words;
 };
 template <int C>
-__device__ __forceinline__ Place place_of(int cw) {
+__device__ __forceinline__ Place place_of(int cw, int block_words) {
   const int warp = threadIdx.x >> 5;
   Place p;
   p.part = warp & (cw - 1);
   p.group = warp / cw;
   p.col0 = p.part * 32 * C + (threadIdx.x & 31);
-  p.words = WORDS * cw / WARPS;
+  p.words = block_words * cw / WARPS;
   p.word0 = p.group * p.words;
   return p;
 }
 
-// The block's logits of 32 words and MT rows: each warp leaves its columns' share in red[part][row][word].
+// The block's logits of its words and MT rows: each warp leaves its columns' share in red[part][row][word].
 template <int MT, int C>
-__device__ __forceinline__ void dots(const float (&x)[MT][C], const float* __restrict__ w, long long v0, int V, int E, const Place& at, float* red) {
-  constexpr int WS = Words<MT, C>::SUM, WL = Words<MT, C>::LOAD, N = WS * MT;
+__device__ __forceinline__ void dots(const float (&x)[MT][C], const float* __restrict__ w, long long v0, int V, int E, const Place& at, float* red,
+                                     float (&b)[Words<MT, C>::LOAD][C]) {
+  constexpr int WS = Words<MT, C>::SUM, WL = Words<MT, C>::LOAD, WORDS = Words<MT, C>::BLOCK, N = WS * MT;
   const int lane = threadIdx.x & 31;
   const float* col[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) col[c] = w + min(at.col0 + 32 * c, E - 1);        // x is 0 past the last column
 #pragma unroll 1
   for (int s = 0; s < at.words; s += WL) {
-    float b[WL][C];
 #pragma unroll
     for (int i = 0; i < WL; ++i) {
       const long long v = min(v0 + at.word0 + s + i, (long long)V - 1) * E;
@@ -136,7 +139,7 @@ __device__ __forceinline__ void load_rows(float (&x)[MT][C], const float* __rest
 // Row t's (m log2 e, s) from the blocks' partial ones, by `lanes` lanes of a warp that stand together.
 __device__ __forceinline__ float2 join_parts(const float2* partial, int parts, long long M, long long t, int l, int lanes) {
   float m = -INFINITY, s = 0.0f;
-#pragma unroll 4
+#pragma unroll 8
   for (int j = l; j < parts; j += lanes) {
     const float2 b = __ldcg(partial + (long long)j * M + t);
     const float top = fmaxf(m, b.x);
@@ -152,12 +155,13 @@ __device__ __forceinline__ float2 join_parts(const float2* partial, int parts, l
 }
 
 template <int MT, int C>
-__global__ void __launch_bounds__(THREADS) few_rows_forward_kernel(const Rows a) {
+__global__ void __launch_bounds__(THREADS, MT > 1 ? 1 : C < 4 ? 3 : 2) few_rows_forward_kernel(const Rows a) {
   const LmRows& p = a.r;
+  constexpr int WORDS = Words<MT, C>::BLOCK;
   __shared__ float red[2][WARPS][MT * WORDS];
   __shared__ int last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Place at = place_of<C>(p.cw);
+  const Place at = place_of<C>(p.cw, WORDS);
   const int m0 = blockIdx.y * MT;
   float x[MT][C];
   load_rows<MT, C>(x, p.x, m0, p.M, p.E, at.col0, nullptr);
@@ -168,15 +172,16 @@ __global__ void __launch_bounds__(THREADS) few_rows_forward_kernel(const Rows a)
   const float l2 = 1.4426950408889634f / p.T;
   int buf = 0;
   for (long long v0 = (long long)blockIdx.x * WORDS; v0 < p.V; v0 += (long long)gridDim.x * WORDS, buf ^= 1) {
-    dots<MT, C>(x, p.w, v0, p.V, p.E, at, red[buf][at.part]);
+    float b[Words<MT, C>::LOAD][C];
+    dots<MT, C>(x, p.w, v0, p.V, p.E, at, red[buf][at.part], b);
     __syncthreads();                                            // the other buffer is free: its readers passed this barrier
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
       const int r = warp + i * WARPS;
       if (r < MT) {
         float z = 0.0f;
-        for (int k = 0; k < p.cw; ++k) z += red[buf][k][r * WORDS + lane];
-        z = v0 + lane < p.V ? z * l2 : -INFINITY;
+        for (int k = 0; k < p.cw; ++k) z += red[buf][k][r * WORDS + (lane & (WORDS - 1))];
+        z = lane < WORDS && v0 + lane < p.V ? z * l2 : -INFINITY;
         const float top = fmaxf(m[i], warp_max(z));
         if (top != -INFINITY) {
           s[i] = s[i] * gt_ex2(m[i] - top) + warp_sum(gt_ex2(z - top));
@@ -201,6 +206,41 @@ __global__ void __launch_bounds__(THREADS) few_rows_forward_kernel(const Rows a)
   __syncthreads();
   if (!last) return;
   __threadfence();
+  if (MT == 1) {                                                // one row: the whole block
+    __shared__ float zs[WARPS];
+    __shared__ float2 ms[WARPS];
+    const float f = p.targets[0];
+    const bool in_range = f >= 0.0f && f < (float)p.V, used = f != p.ignore && in_range;
+    const float* wr = p.w + (long long)(used ? (int)f : 0) * p.E;
+    float z = 0.0f;
+#pragma unroll 4
+    for (int e = threadIdx.x; e < p.E; e += THREADS) z = fmaf(p.x[e], wr[e], z);
+    float2 st = join_parts(p.partial + warp * 32, max(0, min(32, (int)gridDim.x - warp * 32)), 1, 0, lane, 32);
+    for (int j = warp * 32 + THREADS; j < (int)gridDim.x; j += THREADS) {
+      const float2 more = join_parts(p.partial + j, min(32, (int)gridDim.x - j), 1, 0, lane, 32);
+      const float top = fmaxf(st.x, more.x);
+      st = top == -INFINITY ? make_float2(top, st.y + more.y) : make_float2(top, st.y * gt_ex2(st.x - top) + more.y * gt_ex2(more.x - top));
+    }
+    z = warp_sum(z);
+    if (lane == 0) { zs[warp] = z; ms[warp] = st; }
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    for (int k = 1; k < WARPS; ++k) {
+      z += zs[k];
+      const float2 more = ms[k];
+      const float top = fmaxf(st.x, more.x);
+      st = top == -INFINITY ? make_float2(top, st.y + more.y) : make_float2(top, st.y * gt_ex2(st.x - top) + more.y * gt_ex2(more.x - top));
+    }
+    const float loss = used ? logf(st.y) - (z - st.x * 0.6931471805599453f) : 0.0f;
+    if (f != p.ignore && !in_range) atomicExch(a.status, GT_ERR_INVALID_ARG);
+    p.s.stats[0] = st;
+    p.s.ids[0] = used ? (int)f : LM_UNUSED;
+    p.s.q[0] = p.s.weight[0] = used ? 1.0f : 0.0f;
+    p.s.scalars->count = used ? 1 : 0;
+    if (p.row_loss) p.row_loss[0] = loss;
+    if (p.loss) *p.loss = loss;
+    return;
+  }
   // a row by a warp, or by eight lanes where rows are short: four rows a warp then, with their loads in flight together
   const int lanes = p.E <= 256 ? 8 : 32, l = lane & (lanes - 1), per_block = THREADS / lanes;
   double total = 0.0;
@@ -213,7 +253,7 @@ __global__ void __launch_bounds__(THREADS) few_rows_forward_kernel(const Rows a)
     const float* xr = p.x + (long long)(used ? t : 0) * p.E;
     const float* wr = p.w + (long long)(used ? (int)f : 0) * p.E;
     float z = 0.0f;
-#pragma unroll 8
+#pragma unroll 24
     for (int e = l; e < p.E; e += lanes) z = fmaf(xr[e], wr[e], z);
     const float2 st = join_parts(p.partial, gridDim.x, p.M, row ? t : 0, l, lanes);
     for (int o = lanes / 2; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
@@ -248,14 +288,15 @@ __global__ void __launch_bounds__(THREADS) few_rows_forward_kernel(const Rows a)
 }
 
 template <int MT, int C>
-__global__ void __launch_bounds__(THREADS) few_rows_backward_kernel(const Rows a) {
+__global__ void __launch_bounds__(THREADS, MT > 1 ? 1 : C < 4 ? 3 : 2) few_rows_backward_kernel(const Rows a) {
   const LmRows& p = a.r;
+  constexpr int WORDS = Words<MT, C>::BLOCK;
   // the warps' shares of the logits; at the end, dx of half the groups of warps (4 x 32 columns a lane a warp, 4 warps)
   __shared__ float pool[MT * 512 > WARPS * MT * WORDS ? MT * 512 : WARPS * MT * WORDS];
   float (*const red)[MT * WORDS] = reinterpret_cast<float (*)[MT * WORDS]>(pool);
   __shared__ __align__(16) float gs[WORDS * MT];                // G, word by word
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Place at = place_of<C>(p.cw);
+  const Place at = place_of<C>(p.cw, WORDS);
   const float l2 = 1.4426950408889634f / p.T;
   constexpr int ROWS = (MT + WARPS - 1) / WARPS;
   for (int m0 = 0; m0 < p.M; m0 += MT) {
@@ -279,14 +320,15 @@ __global__ void __launch_bounds__(THREADS) few_rows_backward_kernel(const Rows a
       }
     }
     for (long long v0 = (long long)blockIdx.x * WORDS; v0 < p.V; v0 += (long long)gridDim.x * WORDS) {
-      dots<MT, C>(x, p.w, v0, p.V, p.E, at, red[at.part]);
+      float kept[Words<MT, C>::LOAD][C];
+      dots<MT, C>(x, p.w, v0, p.V, p.E, at, red[at.part], kept);
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < ROWS; ++i) {
         const int r = warp + i * WARPS;
         if (r < MT) {
           float z = 0.0f;
-          for (int k = 0; k < p.cw; ++k) z += red[k][r * WORDS + lane];
+          for (int k = 0; k < p.cw; ++k) z += red[k][r * WORDS + (lane & (WORDS - 1))];
           const int t = m0 + r, v = (int)v0 + lane;
           float g = 0.0f;
           if (t < p.M && p.s.weight[t] != 0.0f && v < p.V) {
@@ -296,15 +338,17 @@ __global__ void __launch_bounds__(THREADS) few_rows_backward_kernel(const Rows a
             while (lo < hi) { const int mid = (lo + hi) >> 1; if (ids[mid] < v) lo = mid + 1; else hi = mid; }
             for (; lo < p.K && ids[lo] == v; ++lo) g -= cq[i] * p.s.q[(long long)t * p.K + lo];
           }
-          gs[lane * MT + r] = g;
+          if (lane < WORDS) gs[lane * MT + r] = g;
         }
       }
       __syncthreads();
       const int words = min(at.words, (int)min((long long)WORDS, p.V - v0) - at.word0);
       const bool add = p.acc_dw || m0 > 0;
       constexpr int GROUP = 4;                                  // words whose loads go out together, ahead of the stores
-#pragma unroll 1
-      for (int i0 = 0; i0 < words; i0 += GROUP) {
+      constexpr bool KEPT = Words<MT, C>::KEPT;
+#pragma unroll(KEPT ? WORDS / GROUP : 1)
+      for (int i0 = 0; i0 < (KEPT ? WORDS : words); i0 += GROUP) {
+        if (KEPT && i0 >= words) break;
         float b[GROUP][C], d[GROUP][C];
 #pragma unroll
         for (int i = 0; i < GROUP; ++i) {
@@ -312,7 +356,7 @@ __global__ void __launch_bounds__(THREADS) few_rows_backward_kernel(const Rows a
 #pragma unroll
           for (int c = 0; c < C; ++c) {
             const int col = min(at.col0 + 32 * c, p.E - 1);
-            b[i][c] = p.dx_part ? __ldg(p.w + row + col) : 0.0f;        // read a moment ago: in L1
+            b[i][c] = Words<MT, C>::KEPT ? kept[i % Words<MT, C>::LOAD][c] : p.dx_part ? __ldg(p.w + row + col) : 0.0f;
             d[i][c] = add && p.dw ? p.dw[row + col] : 0.0f;
           }
         }
@@ -427,13 +471,15 @@ int launch(gt_ctx* ctx, const LmRows& p, bool backward) {
 
 }  // namespace
 
+// Measured against the tensor-core path, with gradients, us (this / that): 8 x 768 x 50257 359 / 366, 16 x 768 x 50257 370 / 366,
+// 16 x 256 x 8000 77 / 106, 64 x 128 x 4000 76 / 81, 64 x 256 x 4000 78 / 82, 64 x 512 x 4000 135 / 91, 128 x 128 x 4000 112 / 81.
 bool gt_lm_few_rows(long long M, long long V, long long E) {
   if (E > 1024) return false;
-  return M <= 16 || (M <= 256 && M * V * E <= LM_ROWS_WORK);
+  return M <= 16 || (M <= 64 && M * V * E <= LM_ROWS_WORK);
 }
 
 int gt_lm_rows_parts(gt_ctx* ctx, long long M, long long V, bool backward) {
-  const long long blocks = (V + WORDS - 1) / WORDS, tiles = M <= 16 ? 1 : (M + 15) / 16;
+  const long long words = M == 1 ? 16 : 32, blocks = (V + words - 1) / words, tiles = M <= 16 ? 1 : (M + 15) / 16;
   long long most = (M <= 1 ? 3ll : 2ll) * ctx->sm_count;         // blocks an SM; one row: 138 us with two, 130 with three, 137 with four
   if (!backward) most = (most + tiles - 1) / tiles;
   return (int)(blocks < most ? blocks : most);
