@@ -91,6 +91,7 @@ struct Rows {
   float* loss;                             // null: the rows' losses are what is asked for
   const float* upstream;                   // backward only; forward gradients are for an upstream gradient of 1
   int reduction, accumulate;
+  unsigned long long* ticket;
 };
 
 __device__ __forceinline__ float row_factor(const Rows& p, long long t) {
@@ -104,11 +105,8 @@ __device__ __forceinline__ float row_factor(const Rows& p, long long t) {
 __device__ __forceinline__ void finish(const Rows& p, double* red) {
   __shared__ int last;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    __threadfence();
-    last = atomicAdd(&p.s.scalars->done, 1) == (int)gridDim.x - 1;
-    __threadfence();
-  }
+  unsigned none;
+  if (threadIdx.x == 0) last = lm_count_out(p.ticket, gridDim.x, 0, &none);
   __syncthreads();
   if (!last) return;
   double a = 0.0;
@@ -405,6 +403,7 @@ extern "C" int gt_topk_distillation(gt_ctx* ctx, float* loss, void* saved, float
   p.row_loss = reduction == GT_REDUCE_NONE ? loss : (float*)((char*)saved + p.s.bytes);
   p.loss = reduction == GT_REDUCE_NONE ? nullptr : loss;
   p.reduction = reduction;
+  p.ticket = lm_ticket(ctx);
   int rc = gt_lm_top_targets(ctx, p.s, p.row_loss, ids, teacher, B, C, K, temperature);
   if (rc != GT_OK) return rc;
   // The row in shared memory: with a gradient, for rows long enough to be worth a block of 1024 threads and short enough to fit

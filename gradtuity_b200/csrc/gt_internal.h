@@ -20,7 +20,8 @@ struct gt_ctx {
   int sm_count;
   cudaStream_t stream;        // compute stream (non-blocking)
   int* d_status;              // device status word written by bounded waits that ran out; the allocation is 4 KB:
-                              // ints 16..271 are the "C tile zeroed" flags of the GEMM's last-wave split
+                              // ints 16..271 are the "C tile zeroed" flags of the GEMM's last-wave split,
+                              // 1016..1019 the tickets of the language-model losses (lm_ticket)
   int tail_epoch;             // value those flags take in the next launch that uses them
   int* d_sched;               // ring of GT_SCHED_RING work-unit counters for dynamically scheduled launches (zero when idle)
   long long sched_seq;        // launches that took a counter so far

@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(1024) hard_targets_kernel(const float* __restr
   }
   if (threadIdx.x == 0) {
     *counters = 0;
-    s.scalars->count = base; s.scalars->done = 0; s.scalars->amax_x = 0; s.scalars->amax_w = 0;
+    s.scalars->count = base; s.scalars->amax_x = 0; s.scalars->amax_w = 0;
   }
 }
 
@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(1024) hard_targets_kernel(const float* __restr
 // counting, for each place, the places that go before it (K^2 comparisons, K is tens to a few hundred).
 __global__ void __launch_bounds__(128) top_targets_kernel(const float* __restrict__ ids, const float* __restrict__ teacher, long long M,
                                                           long long V, int K, float inv_T, LmSaved s,
-                                                          float* __restrict__ row_loss, int* status) {
+                                                          float* __restrict__ row_loss, unsigned long long* ticket, int* status) {
   extern __shared__ float smem[];
   const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
   int* key = reinterpret_cast<int*>(smem) + (size_t)w * 2 * K;
@@ -97,8 +97,7 @@ __global__ void __launch_bounds__(128) top_targets_kernel(const float* __restric
   const long long t = (long long)blockIdx.x * 4 + w;
   float mx = -INFINITY;
   bool any = false;
-  if (t >= M) return;
-  {
+  if (t < M) {
     for (int k = l; k < K; k += 32) {
       const float f = ids[t * K + k], v = teacher[t * K + k];
       bool used = !(f < 0.0f) && v > -INFINITY;
@@ -145,10 +144,12 @@ __global__ void __launch_bounds__(128) top_targets_kernel(const float* __restric
     if (l == 0) {
       s.weight[t] = any ? 1.0f : 0.0f;
       s.konst[t] = konst;
-      if (any) atomicAdd(&s.scalars->count, 1);             // whole numbers: the order does not matter
-      else row_loss[t] = 0.0f;
+      if (!any) row_loss[t] = 0.0f;
     }
   }
+  const int n = __syncthreads_count(any && l == 0);
+  unsigned sum;
+  if (threadIdx.x == 0 && lm_count_out(ticket, gridDim.x, n, &sum)) s.scalars->count = (int)sum;
 }
 
 // The same for a distillation's rows, whose targets are there.
@@ -158,7 +159,7 @@ __global__ void __launch_bounds__(1024) compact_rows_kernel(long long M, LmSaved
     const long long t = t0 + threadIdx.x;
     append_rows(t < M && s.weight[t] != 0.0f, t, base, s.row_of);
   }
-  if (threadIdx.x == 0) { *counters = 0; s.scalars->count = base; }
+  if (threadIdx.x == 0) { *counters = 0; s.scalars->count = base; s.scalars->amax_x = 0; s.scalars->amax_w = 0; }
 }
 
 // ---- operands of the linear forms: largest value, then the split into halves ------------------------
@@ -288,7 +289,7 @@ __global__ void __launch_bounds__(1024) join_stats_kernel(const float2* __restri
 // row's targets.  The last block to end adds the rows' losses up, in 64 bits and in a fixed order.
 template <int WARPS_A_ROW>
 __global__ void __launch_bounds__(256) target_loss_kernel(float* __restrict__ row_loss, float* __restrict__ loss, const float* __restrict__ x,
-                                                          const float* __restrict__ w, long long M, int E, int K, float T, int mean, int by_row, LmSaved s) {
+                                                          const float* __restrict__ w, long long M, int E, int K, float T, int mean, int by_row, LmSaved s, unsigned long long* ticket) {
   __shared__ float part[8];
   __shared__ double sums[8];
   __shared__ int last;
@@ -334,7 +335,8 @@ __global__ void __launch_bounds__(256) target_loss_kernel(float* __restrict__ ro
   if (!loss) return;
   __threadfence();
   __syncthreads();
-  if (threadIdx.x == 0) last = atomicAdd(&s.scalars->done, 1) == (int)gridDim.x - 1;
+  unsigned none;
+  if (threadIdx.x == 0) last = lm_count_out(ticket, gridDim.x, 0, &none);
   __syncthreads();
   if (!last) return;
   __threadfence();
@@ -501,8 +503,8 @@ int finish_rows(gt_ctx* ctx, float* row_loss, float* loss, const float2* partial
   float* out = reduction == GT_REDUCE_NONE ? nullptr : loss;
   const int mean = reduction == GT_REDUCE_MEAN;
   join_stats_kernel<<<(unsigned)((M + 31) / 32), 1024, 0, ctx->stream>>>(partial, parts, M, by_row, s);
-  if (K == 1) target_loss_kernel<1><<<(unsigned)((M + 7) / 8), 256, 0, ctx->stream>>>(row_loss, out, x, w, M, (int)E, (int)K, T, mean, by_row, s);
-  else target_loss_kernel<8><<<(unsigned)M, 256, 0, ctx->stream>>>(row_loss, out, x, w, M, (int)E, (int)K, T, mean, by_row, s);
+  if (K == 1) target_loss_kernel<1><<<(unsigned)((M + 7) / 8), 256, 0, ctx->stream>>>(row_loss, out, x, w, M, (int)E, (int)K, T, mean, by_row, s, lm_ticket(ctx));
+  else target_loss_kernel<8><<<(unsigned)M, 256, 0, ctx->stream>>>(row_loss, out, x, w, M, (int)E, (int)K, T, mean, by_row, s, lm_ticket(ctx));
   GT_CUDA_OK(ctx, cudaGetLastError());
   ctx->launches += 2;
   return GT_OK;
@@ -516,12 +518,12 @@ int linear_forward(gt_ctx* ctx, float* loss, void* saved, void* scratch, const f
   if (l.few_rows) {
     LmRows r = rows_problem(l, x, w, M, V, E, K, T, reduction);
     r.parts = gt_lm_rows_parts(ctx, M, V, false);
+    r.ticket = lm_ticket(ctx);
     if (!targets) {
       int rc = prepare_linear(ctx, s, l.p.counters, rows, nullptr, 0.0f, ids, teacher, M, V, K, T);
       if (rc == GT_OK) rc = gt_lm_rows_forward(ctx, r);
       return rc != GT_OK ? rc : finish_rows(ctx, rows, loss, l.p.partial, r.parts, x, w, M, E, K, T, reduction, 1, s);
     }
-    GT_CUDA_OK(ctx, cudaMemsetAsync(s.scalars, 0, sizeof(LmScalars), ctx->stream));
     r.targets = targets; r.ignore = ignore;
     r.row_loss = rows;
     r.loss = reduction == GT_REDUCE_NONE ? nullptr : loss;
@@ -545,8 +547,8 @@ int linear_forward(gt_ctx* ctx, float* loss, void* saved, void* scratch, const f
 
 int gt_lm_top_targets(gt_ctx* ctx, const LmSaved& s, float* row_loss, const float* ids, const float* teacher, long long M, long long V, long long K,
                       float T) {
-  GT_CUDA_OK(ctx, cudaMemsetAsync(s.scalars, 0, sizeof(LmScalars), ctx->stream));
-  top_targets_kernel<<<(unsigned)((M + 3) / 4), 128, (size_t)4 * 2 * K * 4, ctx->stream>>>(ids, teacher, M, V, (int)K, 1.0f / T, s, row_loss, ctx->d_status);
+  top_targets_kernel<<<(unsigned)((M + 3) / 4), 128, (size_t)4 * 2 * K * 4, ctx->stream>>>(ids, teacher, M, V, (int)K, 1.0f / T, s, row_loss, lm_ticket(ctx),
+                                                                                          ctx->d_status);
   GT_CUDA_OK(ctx, cudaGetLastError());
   ctx->launches += 1;
   return GT_OK;

@@ -10,12 +10,28 @@ constexpr int LM_UNUSED = 0x7fffffff;        // id of a place that is not in use
 // Values that a call computes on the device and later launches of it read.
 struct LmScalars {
   int count;            // rows that count
-  int done;             // blocks of a rows' kernel that have ended
   unsigned amax_x;      // largest finite |x|, |w| as float bits (whole-number maximum: the order does not matter)
   unsigned amax_w;
   float logit2;         // log2(e) / T times the operands' scales: accumulator -> z log2(e)
   float dx, dw;         // accumulator -> dx, dw
 };
+
+// A word in which the blocks of a launch count themselves out, so that the last one can go on with what all have written: zero
+// between launches, the last block sees to that.  One for each stream that the context launches on.
+inline unsigned long long* lm_ticket(gt_ctx* ctx) { return (unsigned long long*)(ctx->d_status + 1016 + (ctx->side_saved ? 2 : 0)); }
+#ifdef __CUDACC__
+// Called by one thread of each block once the block's writes are done (behind a barrier).  True in the last block of `blocks`; `sum` is
+// then the sum of all blocks' `mine` (whole numbers: the order does not matter).
+__device__ __forceinline__ bool lm_count_out(unsigned long long* ticket, unsigned blocks, unsigned mine, unsigned* sum) {
+  __threadfence();
+  const unsigned long long was = atomicAdd(ticket, (1ull << 32) + mine);
+  if ((unsigned)(was >> 32) != blocks - 1) return false;
+  *ticket = 0;
+  __threadfence();
+  *sum = (unsigned)was + mine;
+  return true;
+}
+#endif
 
 // What the forward pass leaves for the backward pass, in one block of memory.
 struct LmSaved {
@@ -107,6 +123,7 @@ struct LmRows {
   const float* upstream; int reduction;
   float* dw; int acc_dw;
   float* dx_part;                          // (parts, M, E); null: no dx wanted
+  unsigned long long* ticket;
   int cw, c;                               // warps that share the columns, columns a lane
 };
 constexpr long long LM_ROWS_WORK = 64ll << 20;

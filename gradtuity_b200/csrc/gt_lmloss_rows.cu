@@ -202,7 +202,8 @@ __global__ void __launch_bounds__(THREADS, MT > 1 ? 1 : C < 4 ? 3 : 2) few_rows_
   // ---- cross entropy: the last block takes the losses
   __threadfence();
   __syncthreads();
-  if (threadIdx.x == 0) last = atomicAdd(&p.s.scalars->done, 1) == (int)(gridDim.x * gridDim.y) - 1;
+  unsigned none;
+  if (threadIdx.x == 0) last = lm_count_out(p.ticket, gridDim.x * gridDim.y, 0, &none);
   __syncthreads();
   if (!last) return;
   __threadfence();
