@@ -131,6 +131,8 @@ constexpr int STREAM_THREADS = 512;
 
 template <bool BACKWARD>
 __global__ void __launch_bounds__(STREAM_THREADS) distill_rows_kernel(const Rows p) {
+  gt_let_next_kernel_start();
+  gt_wait_for_previous_kernel();
   __shared__ float2 red[STREAM_THREADS / 32];
   __shared__ double sums[STREAM_THREADS / 32];
   const long long t = blockIdx.x;
@@ -233,6 +235,8 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
 }
 
 __global__ void __launch_bounds__(ROW_THREADS, 1) distill_row_in_smem_kernel(const Rows p, int nchunks, int q4, int* status) {
+  gt_let_next_kernel_start();
+  gt_wait_for_previous_kernel();
   extern __shared__ __align__(128) uint8_t row_smem[];
   __shared__ float2 red[32];
   __shared__ double sums[32];
@@ -417,11 +421,10 @@ extern "C" int gt_topk_distillation(gt_ctx* ctx, float* loss, void* saved, float
     if (chunks < 2) chunks = 2;
     if (chunks > ROW_MAX_CHUNKS) chunks = ROW_MAX_CHUNKS;
     const int grid = (int)(B < ctx->sm_count ? B : ctx->sm_count);
-    distill_row_in_smem_kernel<<<grid, ROW_THREADS, (size_t)units * 16, ctx->stream>>>(p, chunks, (units + chunks - 1) / chunks, ctx->d_status);
+    GT_CUDA_OK(ctx, gt_launch_overlapped(distill_row_in_smem_kernel, dim3(grid), dim3(ROW_THREADS), (size_t)units * 16, ctx->stream, p, chunks, (units + chunks - 1) / chunks, ctx->d_status));
   } else {
-    distill_rows_kernel<false><<<(unsigned)B, STREAM_THREADS, 0, ctx->stream>>>(p);
+    GT_CUDA_OK(ctx, gt_launch_overlapped(distill_rows_kernel<false>, dim3((unsigned)B), dim3(STREAM_THREADS), 0, ctx->stream, p));
   }
-  GT_CUDA_OK(ctx, cudaGetLastError());
   ctx->launches += 1;
   return GT_OK;
 }
@@ -437,8 +440,7 @@ extern "C" int gt_topk_distillation_backward(gt_ctx* ctx, float* dlogits, int64_
   p.B = B; p.C = (int)C; p.K = (int)K; p.T = temperature; p.l2 = 1.4426950408889634f / temperature;
   p.s = lm_saved(saved, B, K);
   p.upstream = upstream; p.reduction = reduction; p.accumulate = accumulate;
-  distill_rows_kernel<true><<<(unsigned)B, STREAM_THREADS, 0, ctx->stream>>>(p);
-  GT_CUDA_OK(ctx, cudaGetLastError());
+  GT_CUDA_OK(ctx, gt_launch_overlapped(distill_rows_kernel<true>, dim3((unsigned)B), dim3(STREAM_THREADS), 0, ctx->stream, p));
   ctx->launches += 1;
   return GT_OK;
 }

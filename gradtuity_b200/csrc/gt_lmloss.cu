@@ -62,6 +62,8 @@ __device__ __forceinline__ void append_rows(bool counts, long long t, int& base,
 // which also clears what later kernels count in.
 __global__ void __launch_bounds__(1024) hard_targets_kernel(const float* __restrict__ targets, long long M, long long V, float ignore, LmSaved s,
                                                             float* __restrict__ row_loss, int* counters, int* status) {
+  gt_let_next_kernel_start();
+  gt_wait_for_previous_kernel();
   int base = 0;
   for (long long t0 = 0; t0 < M; t0 += 1024) {
     const long long t = t0 + threadIdx.x;
@@ -90,6 +92,8 @@ __global__ void __launch_bounds__(1024) hard_targets_kernel(const float* __restr
 __global__ void __launch_bounds__(128) top_targets_kernel(const float* __restrict__ ids, const float* __restrict__ teacher, long long M,
                                                           long long V, int K, float inv_T, LmSaved s,
                                                           float* __restrict__ row_loss, unsigned long long* ticket, int* status) {
+  gt_let_next_kernel_start();
+  gt_wait_for_previous_kernel();
   extern __shared__ float smem[];
   const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
   int* key = reinterpret_cast<int*>(smem) + (size_t)w * 2 * K;
@@ -154,6 +158,8 @@ __global__ void __launch_bounds__(128) top_targets_kernel(const float* __restric
 
 // The same for a distillation's rows, whose targets are there.
 __global__ void __launch_bounds__(1024) compact_rows_kernel(long long M, LmSaved s, int* counters) {
+  gt_let_next_kernel_start();
+  gt_wait_for_previous_kernel();
   int base = 0;
   for (long long t0 = 0; t0 < M; t0 += 1024) {
     const long long t = t0 + threadIdx.x;
@@ -167,6 +173,8 @@ __global__ void __launch_bounds__(1024) compact_rows_kernel(long long M, LmSaved
 // Whole matrix w, and of x the rows that count.  A maximum of bits as whole numbers, so the order of the additions is no matter.
 __global__ void __launch_bounds__(256) largest_kernel(const float* __restrict__ x, const float* __restrict__ w, long long V, long long E, LmSaved s,
                                                       int blocks_x) {
+  gt_let_next_kernel_start();
+  gt_wait_for_previous_kernel();
   const bool is_x = (int)blockIdx.x < blocks_x;
   const long long rows = is_x ? s.scalars->count : V;
   const int first = is_x ? blockIdx.x : blockIdx.x - blocks_x, step = is_x ? blocks_x : gridDim.x - blocks_x;
@@ -210,6 +218,8 @@ __device__ __forceinline__ int scale_exponent(unsigned amax) {
 // A warp per row.  x: compact rows, and zeros behind them to the end of the last tile of rows.
 __global__ void __launch_bounds__(256) split_kernel(const float* __restrict__ x, const float* __restrict__ w, long long M, long long V, long long E,
                                                     long long pitch, LmSaved s, LmSplit xs, LmSplit ws, int products, float T, int blocks_x) {
+  gt_let_next_kernel_start();
+  gt_wait_for_previous_kernel();
   const int l = threadIdx.x & 31;
   const bool is_x = (int)blockIdx.x < blocks_x;
   const int ex = scale_exponent(s.scalars->amax_x), ew = scale_exponent(s.scalars->amax_w);
@@ -257,13 +267,14 @@ __global__ void __launch_bounds__(256) split_kernel(const float* __restrict__ x,
 // ---- rows ------------------------------------------------------------------------------------------
 
 // The linear forms: (m, s) of the rows that count from the parts' (tiles of words, or blocks).  32 rows a block, their parts shared
-// out over 32 warps, so that a warp reads whole lines.  by_row: parts and stats go by row, not by compact row.
-__global__ void __launch_bounds__(1024) join_stats_kernel(const float2* __restrict__ partial, int parts, long long M, int by_row, LmSaved s) {
+// out over 32 warps, so that a warp reads whole lines.
+__global__ void __launch_bounds__(1024) join_stats_kernel(const float2* __restrict__ partial, int parts, long long M, LmSaved s) {
+  gt_let_next_kernel_start();
+  gt_wait_for_previous_kernel();
   __shared__ float2 red[32][33];
   const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
   const long long i = (long long)blockIdx.x * 32 + l;
   const bool live = i < s.scalars->count;
-  const long long at = live && by_row ? s.row_of[i] : i;
   float m = -INFINITY, sum = 0.0f;                            // m in units of log 2
   auto add = [&](float2 b) {
     const float top = fmaxf(m, b.x);
@@ -273,7 +284,7 @@ __global__ void __launch_bounds__(1024) join_stats_kernel(const float2* __restri
   };
   if (live) {
 #pragma unroll 4
-    for (int j = w; j < parts; j += 32) add(partial[(long long)j * M + at]);
+    for (int j = w; j < parts; j += 32) add(partial[(long long)j * M + i]);
   }
   red[w][l] = make_float2(m, sum);
   __syncthreads();
@@ -282,25 +293,50 @@ __global__ void __launch_bounds__(1024) join_stats_kernel(const float2* __restri
   const float top = warp_max(mine.x);
   sum = warp_sum(top == -INFINITY ? mine.y : mine.y * gt_ex2(mine.x - top));
   const long long r = (long long)blockIdx.x * 32 + w;
-  if (l == 0 && r < s.scalars->count) s.stats[by_row ? s.row_of[r] : r] = make_float2(top, sum);
+  if (l == 0 && r < s.scalars->count) s.stats[r] = make_float2(top, sum);
 }
 
-// Losses of the compact rows, from the logits of their targets, taken in 32 bits straight from x and w.  WARPS_A_ROW warps share a
-// row's targets.  The last block to end adds the rows' losses up, in 64 bits and in a fixed order.
+// Losses of the rows, from the logits of their targets, taken in 32 bits straight from x and w.  WARPS_A_ROW warps share a row's targets.
+// The rows are the compact ones, with their statistics there; or, with `partial`, all rows, whose parts' statistics are by row
+// and are joined here (WARPS_A_ROW = 8).  The last block to end adds the rows' losses up, in 64 bits and in a fixed order.
 template <int WARPS_A_ROW>
 __global__ void __launch_bounds__(256) target_loss_kernel(float* __restrict__ row_loss, float* __restrict__ loss, const float* __restrict__ x,
-                                                          const float* __restrict__ w, long long M, int E, int K, float T, int mean, int by_row, LmSaved s, unsigned long long* ticket) {
+                                                          const float* __restrict__ w, long long M, int E, int K, float T, int mean,
+                                                          const float2* __restrict__ partial, int parts, LmSaved s, unsigned long long* ticket) {
+  gt_let_next_kernel_start();
+  gt_wait_for_previous_kernel();
   __shared__ float part[8];
+  __shared__ float2 joined[8];
   __shared__ double sums[8];
   __shared__ int last;
   const int warp = threadIdx.x >> 5, l = threadIdx.x & 31;
   const long long i = (long long)blockIdx.x * (8 / WARPS_A_ROW) + warp / WARPS_A_ROW;
-  const bool live = i < s.scalars->count;
+  const bool live = partial ? s.weight[i] != 0.0f : i < s.scalars->count;
   long long t = 0;
   float cross = 0.0f;
+  float2 st = make_float2(0.0f, 1.0f);
+  if (WARPS_A_ROW == 8 && partial) {
+    float m = -INFINITY, sum = 0.0f;
+    auto add = [&](float2 b) {
+      const float top = fmaxf(m, b.x);
+      if (top == -INFINITY) { sum += b.y; return; }
+      sum = sum * gt_ex2(m - top) + b.y * gt_ex2(b.x - top);
+      m = top;
+    };
+    for (int j = threadIdx.x; j < parts; j += 256) add(partial[(long long)j * M + i]);
+    const float top = warp_max(m);
+    sum = warp_sum(top == -INFINITY ? sum : sum * gt_ex2(m - top));
+    if (l == 0) joined[warp] = make_float2(top, sum);
+    __syncthreads();
+    m = -INFINITY; sum = 0.0f;
+    for (int k = 0; k < 8; ++k) add(joined[k]);
+    st = make_float2(m, sum);
+    if (threadIdx.x == 0) s.stats[i] = st;
+  } else if (live) {
+    st = s.stats[i];
+  }
   if (live) {
-    t = s.row_of[i];
-    const float2 st = s.stats[by_row ? t : i];
+    t = partial ? i : s.row_of[i];
     const float log_s = logf(st.y), top = st.x * 0.6931471805599453f;
     const float* xr = x + t * E;
     const bool vec = ((uintptr_t)x & 15) == 0 && ((uintptr_t)w & 15) == 0 && E % 4 == 0;
@@ -358,6 +394,8 @@ __global__ void __launch_bounds__(256) target_loss_kernel(float* __restrict__ ro
 // also clears the steps' counters.  The other blocks (if any): zeros for dx of the rows that do not count, a warp per row.
 __global__ void __launch_bounds__(1024) begin_backward_kernel(const float* __restrict__ upstream, int reduction, float T, LmSaved s, int* counters,
                                                               int steps, float* __restrict__ dx, long long M, long long E) {
+  gt_let_next_kernel_start();
+  gt_wait_for_previous_kernel();
   if (blockIdx.x > 0) {
     for (long long t = (long long)(blockIdx.x - 1) * 32 + (threadIdx.x >> 5); t < M; t += (long long)(gridDim.x - 1) * 32)
       if (s.weight[t] == 0.0f)
@@ -396,6 +434,8 @@ __global__ void __launch_bounds__(1024) begin_backward_kernel(const float* __res
 // dx (+)= the shares of a piece, in order.
 __global__ void __launch_bounds__(256) add_shares_kernel(float* __restrict__ dx, const float* __restrict__ shares, int n_shares, long long M, long long E,
                                                          int add, LmSaved s) {
+  gt_let_next_kernel_start();
+  gt_wait_for_previous_kernel();
   const long long i = blockIdx.x;
   if (i >= s.scalars->count) return;
   float* to = dx + (long long)s.row_of[i] * E;
@@ -430,7 +470,6 @@ Linear linear_layout(gt_ctx* ctx, void* saved, void* scratch, long long M, long 
     LmCarve c = {(char*)saved, 0}, f = {(char*)scratch, 0};
     l.s = lm_saved(c, M, K);
     l.saved_bytes = c.at;
-    p.counters = f.take<int>(1);
     LmCarve b = f;
     l.row_loss = f.take<float>(M);
     p.partial = f.take<float2>((size_t)gt_lm_rows_parts(ctx, M, V, false) * M);
@@ -487,25 +526,31 @@ LmRows rows_problem(const Linear& l, const float* x, const float* w, long long M
 int prepare_linear(gt_ctx* ctx, const LmSaved& s, int* counters, float* row_loss, const float* targets, float ignore, const float* ids,
                    const float* teacher, long long M, long long V, long long K, float T) {
   if (targets) {
-    hard_targets_kernel<<<1, 1024, 0, ctx->stream>>>(targets, M, V, ignore, s, row_loss, counters, ctx->d_status);
+    GT_CUDA_OK(ctx, gt_launch_overlapped(hard_targets_kernel, dim3(1), dim3(1024), 0, ctx->stream, targets, M, V, ignore, s, row_loss, counters, ctx->d_status));
   } else {
     int rc = gt_lm_top_targets(ctx, s, row_loss, ids, teacher, M, V, K, T);
     if (rc != GT_OK) return rc;
-    compact_rows_kernel<<<1, 1024, 0, ctx->stream>>>(M, s, counters);
+    GT_CUDA_OK(ctx, gt_launch_overlapped(compact_rows_kernel, dim3(1), dim3(1024), 0, ctx->stream, M, s, counters));
   }
-  GT_CUDA_OK(ctx, cudaGetLastError());
   ctx->launches += 1;
   return GT_OK;
 }
 
 int finish_rows(gt_ctx* ctx, float* row_loss, float* loss, const float2* partial, int parts, const float* x, const float* w, long long M,
-                long long E, long long K, float T, int reduction, int by_row, const LmSaved& s) {
+                long long E, long long K, float T, int reduction, bool by_row, const LmSaved& s) {
   float* out = reduction == GT_REDUCE_NONE ? nullptr : loss;
   const int mean = reduction == GT_REDUCE_MEAN;
-  join_stats_kernel<<<(unsigned)((M + 31) / 32), 1024, 0, ctx->stream>>>(partial, parts, M, by_row, s);
-  if (K == 1) target_loss_kernel<1><<<(unsigned)((M + 7) / 8), 256, 0, ctx->stream>>>(row_loss, out, x, w, M, (int)E, (int)K, T, mean, by_row, s, lm_ticket(ctx));
-  else target_loss_kernel<8><<<(unsigned)M, 256, 0, ctx->stream>>>(row_loss, out, x, w, M, (int)E, (int)K, T, mean, by_row, s, lm_ticket(ctx));
-  GT_CUDA_OK(ctx, cudaGetLastError());
+  if (by_row) {
+    GT_CUDA_OK(ctx, gt_launch_overlapped(target_loss_kernel<8>, dim3((unsigned)M), dim3(256), 0, ctx->stream, row_loss, out, x, w, M, (int)E, (int)K, T, mean,
+                                         partial, parts, s, lm_ticket(ctx)));
+    ctx->launches += 1;
+    return GT_OK;
+  }
+  GT_CUDA_OK(ctx, gt_launch_overlapped(join_stats_kernel, dim3((unsigned)((M + 31) / 32)), dim3(1024), 0, ctx->stream, partial, parts, M, s));
+  void (*kernel)(float*, float*, const float*, const float*, long long, int, int, float, int, const float2*, int, LmSaved, unsigned long long*) =
+      K == 1 ? target_loss_kernel<1> : target_loss_kernel<8>;
+  GT_CUDA_OK(ctx, gt_launch_overlapped(kernel, dim3((unsigned)(K == 1 ? (M + 7) / 8 : M)), dim3(256), 0, ctx->stream, row_loss, out, x, w, M, (int)E, (int)K, T, mean,
+                                       (const float2*)nullptr, 0, s, lm_ticket(ctx)));
   ctx->launches += 2;
   return GT_OK;
 }
@@ -520,9 +565,9 @@ int linear_forward(gt_ctx* ctx, float* loss, void* saved, void* scratch, const f
     r.parts = gt_lm_rows_parts(ctx, M, V, false);
     r.ticket = lm_ticket(ctx);
     if (!targets) {
-      int rc = prepare_linear(ctx, s, l.p.counters, rows, nullptr, 0.0f, ids, teacher, M, V, K, T);
+      int rc = gt_lm_top_targets(ctx, s, rows, ids, teacher, M, V, K, T);
       if (rc == GT_OK) rc = gt_lm_rows_forward(ctx, r);
-      return rc != GT_OK ? rc : finish_rows(ctx, rows, loss, l.p.partial, r.parts, x, w, M, E, K, T, reduction, 1, s);
+      return rc != GT_OK ? rc : finish_rows(ctx, rows, loss, l.p.partial, r.parts, x, w, M, E, K, T, reduction, true, s);
     }
     r.targets = targets; r.ignore = ignore;
     r.row_loss = rows;
@@ -534,22 +579,19 @@ int linear_forward(gt_ctx* ctx, float* loss, void* saved, void* scratch, const f
   const long long most = 8ll * ctx->sm_count;
   auto blocks = [&](long long n) { return (int)((n + 7) / 8 < most ? (n + 7) / 8 : most); };
   const int bx = blocks(M), bw = blocks(V);
-  largest_kernel<<<(unsigned)(bx + bw), 256, 0, ctx->stream>>>(x, w, V, E, s, bx);
-  split_kernel<<<(unsigned)(bx + bw), 256, 0, ctx->stream>>>(x, w, M, V, E, l.p.pitch_e, s, l.p.x, l.p.w, l.p.products, T, bx);
-  GT_CUDA_OK(ctx, cudaGetLastError());
+  GT_CUDA_OK(ctx, gt_launch_overlapped(largest_kernel, dim3((unsigned)(bx + bw)), dim3(256), 0, ctx->stream, x, w, V, E, s, bx));
+  GT_CUDA_OK(ctx, gt_launch_overlapped(split_kernel, dim3((unsigned)(bx + bw)), dim3(256), 0, ctx->stream, x, w, M, V, E, l.p.pitch_e, s, l.p.x, l.p.w, l.p.products, T, bx));
   ctx->launches += 2;
   rc = gt_lm_stats(ctx, l.p);
   if (rc != GT_OK) return rc;
-  return finish_rows(ctx, rows, loss, l.p.partial, (int)((V + LM_TILE - 1) / LM_TILE * 2), x, w, M, E, K, T, reduction, 0, s);
+  return finish_rows(ctx, rows, loss, l.p.partial, (int)((V + LM_TILE - 1) / LM_TILE * 2), x, w, M, E, K, T, reduction, false, s);
 }
 
 }  // namespace
 
 int gt_lm_top_targets(gt_ctx* ctx, const LmSaved& s, float* row_loss, const float* ids, const float* teacher, long long M, long long V, long long K,
                       float T) {
-  top_targets_kernel<<<(unsigned)((M + 3) / 4), 128, (size_t)4 * 2 * K * 4, ctx->stream>>>(ids, teacher, M, V, (int)K, 1.0f / T, s, row_loss, lm_ticket(ctx),
-                                                                                          ctx->d_status);
-  GT_CUDA_OK(ctx, cudaGetLastError());
+  GT_CUDA_OK(ctx, gt_launch_overlapped(top_targets_kernel, dim3((unsigned)((M + 3) / 4)), dim3(128), (size_t)4 * 2 * K * 4, ctx->stream, ids, teacher, M, V, (int)K, 1.0f / T, s, row_loss, lm_ticket(ctx), ctx->d_status));
   ctx->launches += 1;
   return GT_OK;
 }
@@ -594,16 +636,14 @@ extern "C" int gt_linear_loss_backward(gt_ctx* ctx, float* dx, float* dw, void* 
   LmProblem& p = l.p;
   p.dx = dx; p.dw = dw; p.acc_dx = acc_dx; p.acc_dw = acc_dw;
   const long long zero_blocks = dx && !acc_dx ? ((M + 31) / 32 < ctx->sm_count ? (M + 31) / 32 : ctx->sm_count) : 0;
-  begin_backward_kernel<<<(unsigned)(1 + zero_blocks), 1024, 0, ctx->stream>>>(upstream, reduction, temperature, l.s, p.counters, l.pieces + 1, dx, M, E);
-  GT_CUDA_OK(ctx, cudaGetLastError());
+  GT_CUDA_OK(ctx, gt_launch_overlapped(begin_backward_kernel, dim3((unsigned)(1 + zero_blocks)), dim3(1024), 0, ctx->stream, upstream, reduction, temperature, l.s, p.counters, l.pieces + 1, dx, M, E));
   ctx->launches += 1;
   for (int piece = 0; piece <= l.pieces; ++piece) {
     int rc = gt_lm_step(ctx, p, piece);
     if (rc != GT_OK) return rc;
     if (piece > 0 && dx && p.dx_split > 1) {
-      add_shares_kernel<<<(unsigned)M, 256, 0, ctx->stream>>>(dx, p.dx_partial, p.dx_split, M, E, acc_dx || piece > 1, l.s);
-      GT_CUDA_OK(ctx, cudaGetLastError());
-      ctx->launches += 1;
+      GT_CUDA_OK(ctx, gt_launch_overlapped(add_shares_kernel, dim3((unsigned)M), dim3(256), 0, ctx->stream, dx, p.dx_partial, p.dx_split, M, E, acc_dx || piece > 1, l.s));
+          ctx->launches += 1;
     }
   }
   return GT_OK;

@@ -2,7 +2,7 @@
 // (and writing dW), and a small problem is launches and latencies; the tensor-core path pays for splitting W into halves first,
 // and for tiles of 256 rows.
 //
-// A block of eight warps takes 32 words at a time (one row: 16).  The E columns are shared out over the lanes of CW warps (1, 2, 4 or 8), C columns
+// One row: a warp per word, in registers for all that is done with it.  More: a block of eight warps takes 32 words at a time.  The E columns are shared out over the lanes of CW warps (1, 2, 4 or 8), C columns
 // each, and the words over the 8 / CW groups of such warps; MT rows of x stay in registers.  Every lane multiplies its columns of a
 // few words with its columns of the rows, the 32 lanes add up by exchanging halves (one exchange per value instead of five), and
 // the warps' sums meet in shared memory.  So W is read once, straight from memory in whole lines, and no operand passes through
@@ -16,7 +16,7 @@
 
 namespace {
 
-constexpr int THREADS = 256, WARPS = 8;
+constexpr int THREADS = 256, WARPS = 8, WORDS = 32;
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -55,11 +55,8 @@ __device__ __forceinline__ void lanes_sum(float (&v)[N]) {
 
 // Words loaded at a time, and multiplied at a time.
 template <int MT, int C> struct Words {
-  static constexpr int SUM = MT == 1 ? 16 : MT == 4 ? 8 : 4;
+  static constexpr int SUM = MT == 4 ? 8 : 4;
   static constexpr int LOAD = MT == 16 && C <= 2 ? 8 : SUM;
-  // A block's words.  One row: few enough for a warp to keep them in registers between the two uses that the backward pass has of them.
-  static constexpr int BLOCK = MT == 1 ? 16 : 32;
-  static constexpr bool KEPT = BLOCK == LOAD;
 };
 
 struct Rows {
@@ -72,28 +69,29 @@ struct Place {
   int part, group, col0, word0, words;
 };
 template <int C>
-__device__ __forceinline__ Place place_of(int cw, int block_words) {
+__device__ __forceinline__ Place place_of(int cw) {
   const int warp = threadIdx.x >> 5;
   Place p;
   p.part = warp & (cw - 1);
   p.group = warp / cw;
   p.col0 = p.part * 32 * C + (threadIdx.x & 31);
-  p.words = block_words * cw / WARPS;
+  p.words = WORDS * cw / WARPS;
   p.word0 = p.group * p.words;
   return p;
 }
 
-// The block's logits of its words and MT rows: each warp leaves its columns' share in red[part][row][word].
+// The block's logits of its words and MT rows: each warp leaves its columns' share in red[row][word].
 template <int MT, int C>
-__device__ __forceinline__ void dots(const float (&x)[MT][C], const float* __restrict__ w, long long v0, int V, int E, const Place& at, float* red,
-                                     float (&b)[Words<MT, C>::LOAD][C]) {
-  constexpr int WS = Words<MT, C>::SUM, WL = Words<MT, C>::LOAD, WORDS = Words<MT, C>::BLOCK, N = WS * MT;
+__device__ __forceinline__ void dots(const float (&x)[MT][C], const float* __restrict__ w, long long v0, int V, int E, const Place& at, float* red) {
+  constexpr int WS = Words<MT, C>::SUM, WL = Words<MT, C>::LOAD, N = WS * MT;
+  static_assert(N >= 32, "every lane holds a sum");
   const int lane = threadIdx.x & 31;
   const float* col[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) col[c] = w + min(at.col0 + 32 * c, E - 1);        // x is 0 past the last column
 #pragma unroll 1
   for (int s = 0; s < at.words; s += WL) {
+    float b[WL][C];
 #pragma unroll
     for (int i = 0; i < WL; ++i) {
       const long long v = min(v0 + at.word0 + s + i, (long long)V - 1) * E;
@@ -114,10 +112,9 @@ __device__ __forceinline__ void dots(const float (&x)[MT][C], const float* __res
         }
       lanes_sum<N>(a);
 #pragma unroll
-      for (int j = 0; j < (N >= 32 ? N / 32 : 1); ++j) {
-        const int k = N >= 32 ? lane * (N / 32) + j : lane * N / 32;             // which sum this lane holds
-        const int word = at.word0 + s + h + k / MT;
-        if (word < WORDS && (N >= 32 || (lane & (32 / (N < 32 ? N : 32) - 1)) == 0)) red[(k % MT) * WORDS + word] = a[j];
+      for (int j = 0; j < N / 32; ++j) {
+        const int k = lane * (N / 32) + j, word = s + h + k / MT;                // which sum this lane holds
+        if (word < at.words) red[(k % MT) * WORDS + at.word0 + word] = a[j];
       }
     }
   }
@@ -155,13 +152,14 @@ __device__ __forceinline__ float2 join_parts(const float2* partial, int parts, l
 }
 
 template <int MT, int C>
-__global__ void __launch_bounds__(THREADS, MT > 1 ? 1 : C < 4 ? 3 : 2) few_rows_forward_kernel(const Rows a) {
+__global__ void __launch_bounds__(THREADS) few_rows_forward_kernel(const Rows a) {
+  gt_let_next_kernel_start();
+  gt_wait_for_previous_kernel();
   const LmRows& p = a.r;
-  constexpr int WORDS = Words<MT, C>::BLOCK;
   __shared__ float red[2][WARPS][MT * WORDS];
   __shared__ int last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Place at = place_of<C>(p.cw, WORDS);
+  const Place at = place_of<C>(p.cw);
   const int m0 = blockIdx.y * MT;
   float x[MT][C];
   load_rows<MT, C>(x, p.x, m0, p.M, p.E, at.col0, nullptr);
@@ -172,16 +170,15 @@ __global__ void __launch_bounds__(THREADS, MT > 1 ? 1 : C < 4 ? 3 : 2) few_rows_
   const float l2 = 1.4426950408889634f / p.T;
   int buf = 0;
   for (long long v0 = (long long)blockIdx.x * WORDS; v0 < p.V; v0 += (long long)gridDim.x * WORDS, buf ^= 1) {
-    float b[Words<MT, C>::LOAD][C];
-    dots<MT, C>(x, p.w, v0, p.V, p.E, at, red[buf][at.part], b);
+    dots<MT, C>(x, p.w, v0, p.V, p.E, at, red[buf][at.part]);
     __syncthreads();                                            // the other buffer is free: its readers passed this barrier
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
       const int r = warp + i * WARPS;
       if (r < MT) {
         float z = 0.0f;
-        for (int k = 0; k < p.cw; ++k) z += red[buf][k][r * WORDS + (lane & (WORDS - 1))];
-        z = lane < WORDS && v0 + lane < p.V ? z * l2 : -INFINITY;
+        for (int k = 0; k < p.cw; ++k) z += red[buf][k][r * WORDS + lane];
+        z = v0 + lane < p.V ? z * l2 : -INFINITY;
         const float top = fmaxf(m[i], warp_max(z));
         if (top != -INFINITY) {
           s[i] = s[i] * gt_ex2(m[i] - top) + warp_sum(gt_ex2(z - top));
@@ -207,41 +204,6 @@ __global__ void __launch_bounds__(THREADS, MT > 1 ? 1 : C < 4 ? 3 : 2) few_rows_
   __syncthreads();
   if (!last) return;
   __threadfence();
-  if (MT == 1) {                                                // one row: the whole block
-    __shared__ float zs[WARPS];
-    __shared__ float2 ms[WARPS];
-    const float f = p.targets[0];
-    const bool in_range = f >= 0.0f && f < (float)p.V, used = f != p.ignore && in_range;
-    const float* wr = p.w + (long long)(used ? (int)f : 0) * p.E;
-    float z = 0.0f;
-#pragma unroll 4
-    for (int e = threadIdx.x; e < p.E; e += THREADS) z = fmaf(p.x[e], wr[e], z);
-    float2 st = join_parts(p.partial + warp * 32, max(0, min(32, (int)gridDim.x - warp * 32)), 1, 0, lane, 32);
-    for (int j = warp * 32 + THREADS; j < (int)gridDim.x; j += THREADS) {
-      const float2 more = join_parts(p.partial + j, min(32, (int)gridDim.x - j), 1, 0, lane, 32);
-      const float top = fmaxf(st.x, more.x);
-      st = top == -INFINITY ? make_float2(top, st.y + more.y) : make_float2(top, st.y * gt_ex2(st.x - top) + more.y * gt_ex2(more.x - top));
-    }
-    z = warp_sum(z);
-    if (lane == 0) { zs[warp] = z; ms[warp] = st; }
-    __syncthreads();
-    if (threadIdx.x != 0) return;
-    for (int k = 1; k < WARPS; ++k) {
-      z += zs[k];
-      const float2 more = ms[k];
-      const float top = fmaxf(st.x, more.x);
-      st = top == -INFINITY ? make_float2(top, st.y + more.y) : make_float2(top, st.y * gt_ex2(st.x - top) + more.y * gt_ex2(more.x - top));
-    }
-    const float loss = used ? logf(st.y) - (z - st.x * 0.6931471805599453f) : 0.0f;
-    if (f != p.ignore && !in_range) atomicExch(a.status, GT_ERR_INVALID_ARG);
-    p.s.stats[0] = st;
-    p.s.ids[0] = used ? (int)f : LM_UNUSED;
-    p.s.q[0] = p.s.weight[0] = used ? 1.0f : 0.0f;
-    p.s.scalars->count = used ? 1 : 0;
-    if (p.row_loss) p.row_loss[0] = loss;
-    if (p.loss) *p.loss = loss;
-    return;
-  }
   // a row by a warp, or by eight lanes where rows are short: four rows a warp then, with their loads in flight together
   const int lanes = p.E <= 256 ? 8 : 32, l = lane & (lanes - 1), per_block = THREADS / lanes;
   double total = 0.0;
@@ -289,15 +251,16 @@ __global__ void __launch_bounds__(THREADS, MT > 1 ? 1 : C < 4 ? 3 : 2) few_rows_
 }
 
 template <int MT, int C>
-__global__ void __launch_bounds__(THREADS, MT > 1 ? 1 : C < 4 ? 3 : 2) few_rows_backward_kernel(const Rows a) {
+__global__ void __launch_bounds__(THREADS) few_rows_backward_kernel(const Rows a) {
+  gt_let_next_kernel_start();
+  gt_wait_for_previous_kernel();
   const LmRows& p = a.r;
-  constexpr int WORDS = Words<MT, C>::BLOCK;
   // the warps' shares of the logits; at the end, dx of half the groups of warps (4 x 32 columns a lane a warp, 4 warps)
   __shared__ float pool[MT * 512 > WARPS * MT * WORDS ? MT * 512 : WARPS * MT * WORDS];
   float (*const red)[MT * WORDS] = reinterpret_cast<float (*)[MT * WORDS]>(pool);
   __shared__ __align__(16) float gs[WORDS * MT];                // G, word by word
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Place at = place_of<C>(p.cw, WORDS);
+  const Place at = place_of<C>(p.cw);
   const float l2 = 1.4426950408889634f / p.T;
   constexpr int ROWS = (MT + WARPS - 1) / WARPS;
   for (int m0 = 0; m0 < p.M; m0 += MT) {
@@ -321,15 +284,14 @@ __global__ void __launch_bounds__(THREADS, MT > 1 ? 1 : C < 4 ? 3 : 2) few_rows_
       }
     }
     for (long long v0 = (long long)blockIdx.x * WORDS; v0 < p.V; v0 += (long long)gridDim.x * WORDS) {
-      float kept[Words<MT, C>::LOAD][C];
-      dots<MT, C>(x, p.w, v0, p.V, p.E, at, red[at.part], kept);
+      dots<MT, C>(x, p.w, v0, p.V, p.E, at, red[at.part]);
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < ROWS; ++i) {
         const int r = warp + i * WARPS;
         if (r < MT) {
           float z = 0.0f;
-          for (int k = 0; k < p.cw; ++k) z += red[k][r * WORDS + (lane & (WORDS - 1))];
+          for (int k = 0; k < p.cw; ++k) z += red[k][r * WORDS + lane];
           const int t = m0 + r, v = (int)v0 + lane;
           float g = 0.0f;
           if (t < p.M && p.s.weight[t] != 0.0f && v < p.V) {
@@ -339,17 +301,15 @@ __global__ void __launch_bounds__(THREADS, MT > 1 ? 1 : C < 4 ? 3 : 2) few_rows_
             while (lo < hi) { const int mid = (lo + hi) >> 1; if (ids[mid] < v) lo = mid + 1; else hi = mid; }
             for (; lo < p.K && ids[lo] == v; ++lo) g -= cq[i] * p.s.q[(long long)t * p.K + lo];
           }
-          if (lane < WORDS) gs[lane * MT + r] = g;
+          gs[lane * MT + r] = g;
         }
       }
       __syncthreads();
       const int words = min(at.words, (int)min((long long)WORDS, p.V - v0) - at.word0);
       const bool add = p.acc_dw || m0 > 0;
       constexpr int GROUP = 4;                                  // words whose loads go out together, ahead of the stores
-      constexpr bool KEPT = Words<MT, C>::KEPT;
-#pragma unroll(KEPT ? WORDS / GROUP : 1)
-      for (int i0 = 0; i0 < (KEPT ? WORDS : words); i0 += GROUP) {
-        if (KEPT && i0 >= words) break;
+#pragma unroll 1
+      for (int i0 = 0; i0 < words; i0 += GROUP) {
         float b[GROUP][C], d[GROUP][C];
 #pragma unroll
         for (int i = 0; i < GROUP; ++i) {
@@ -357,7 +317,7 @@ __global__ void __launch_bounds__(THREADS, MT > 1 ? 1 : C < 4 ? 3 : 2) few_rows_
 #pragma unroll
           for (int c = 0; c < C; ++c) {
             const int col = min(at.col0 + 32 * c, p.E - 1);
-            b[i][c] = Words<MT, C>::KEPT ? kept[i % Words<MT, C>::LOAD][c] : p.dx_part ? __ldg(p.w + row + col) : 0.0f;
+            b[i][c] = p.dx_part ? __ldg(p.w + row + col) : 0.0f;      // read a moment ago: in L1
             d[i][c] = add && p.dw ? p.dw[row + col] : 0.0f;
           }
         }
@@ -366,12 +326,11 @@ __global__ void __launch_bounds__(THREADS, MT > 1 ? 1 : C < 4 ? 3 : 2) few_rows_
           if (i0 + i >= words) break;
           const float* gi = gs + (at.word0 + i0 + i) * MT;
 #pragma unroll
-          for (int m = 0; m < MT; m += MT >= 4 ? 4 : 1) {
+          for (int m = 0; m < MT; m += 4) {
             float g[4];
-            if (MT >= 4) *reinterpret_cast<float4*>(g) = *reinterpret_cast<const float4*>(gi + m);
-            else g[0] = gi[m];
+            *reinterpret_cast<float4*>(g) = *reinterpret_cast<const float4*>(gi + m);
 #pragma unroll
-            for (int k = 0; k < (MT >= 4 ? 4 : 1); ++k)
+            for (int k = 0; k < 4; ++k)
 #pragma unroll
               for (int c = 0; c < C; ++c) {
                 dx[m + k][c] = fmaf(g[k], b[i][c], dx[m + k][c]);
@@ -423,8 +382,188 @@ __global__ void __launch_bounds__(THREADS, MT > 1 ? 1 : C < 4 ? 3 : 2) few_rows_
   }
 }
 
+// ---- one row ------------------------------------------------------------------------------------------
+// A warp takes whole words, two at a time: loads, dot product and, in the backward pass, dx += g w and dW = g x need no other warp, so
+// nothing waits but for memory.  NC: 128 columns each, four a lane; side by side for 16-byte loads (VEC), else 32 apart.
+template <int NC, bool VEC>
+struct Row {
+  float v[NC][4];
+  static __device__ __forceinline__ int column(int i, int j) { return i * 128 + (VEC ? 4 * (threadIdx.x & 31) + j : 32 * j + (threadIdx.x & 31)); }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[i][j] = 0.0f;
+  }
+  __device__ __forceinline__ void load(const float* __restrict__ src, int E) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      if (VEC) {
+        const int col = column(i, 0);
+        const float4 a = col < E ? *reinterpret_cast<const float4*>(src + col) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        v[i][0] = a.x; v[i][1] = a.y; v[i][2] = a.z; v[i][3] = a.w;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[i][j] = column(i, j) < E ? src[column(i, j)] : 0.0f;
+      }
+    }
+  }
+  __device__ __forceinline__ float dot(const Row& o) const {
+    float z = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) z = fmaf(v[i][j], o.v[i][j], z);
+    return z;
+  }
+};
+
+template <int NC, bool VEC>
+__global__ void __launch_bounds__(THREADS) one_row_forward_kernel(const Rows a) {
+  gt_let_next_kernel_start();
+  gt_wait_for_previous_kernel();
+  const LmRows& p = a.r;
+  __shared__ float zs[WARPS];
+  __shared__ float2 ms[WARPS];
+  __shared__ int last;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const float l2 = 1.4426950408889634f / p.T;
+  Row<NC, VEC> x;
+  x.load(p.x, p.E);
+  float m = -INFINITY, s = 0.0f;
+  auto add = [&](float2 b) {
+    const float top = fmaxf(m, b.x);
+    if (top == -INFINITY) { s += b.y; return; }                 // a NaN is no maximum, but it counts
+    s = s * gt_ex2(m - top) + b.y * gt_ex2(b.x - top);
+    m = top;
+  };
+  const int stride = gridDim.x * WARPS;
+  for (int v = blockIdx.x * WARPS + warp; v < p.V; v += 2 * stride) {
+    const bool two = v + stride < p.V;
+    Row<NC, VEC> w0, w1;
+    w0.load(p.w + (long long)v * p.E, p.E);
+    w1.load(p.w + (long long)(two ? v + stride : v) * p.E, p.E);
+    const float z0 = warp_sum(x.dot(w0)) * l2, z1 = warp_sum(x.dot(w1)) * l2;
+    add(make_float2(z0, z0 == z0 ? 1.0f : z0));
+    if (two) add(make_float2(z1, z1 == z1 ? 1.0f : z1));
+  }
+  if (lane == 0) ms[warp] = make_float2(m, s);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int k = 1; k < WARPS; ++k) add(ms[k]);
+    p.partial[blockIdx.x] = make_float2(m, s);
+  }
+  if (!p.targets) return;                                       // distillation: the rows' kernels do the rest
+  unsigned none;
+  if (threadIdx.x == 0) last = lm_count_out(p.ticket, gridDim.x, 0, &none);
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  const float f = p.targets[0];
+  const bool in_range = f >= 0.0f && f < (float)p.V, used = f != p.ignore && in_range;
+  const float* wr = p.w + (long long)(used ? (int)f : 0) * p.E;
+  float z = 0.0f;
+#pragma unroll 4
+  for (int e = threadIdx.x; e < p.E; e += THREADS) z = fmaf(p.x[e], wr[e], z);
+  m = -INFINITY; s = 0.0f;
+#pragma unroll 4
+  for (int j = threadIdx.x; j < (int)gridDim.x; j += THREADS) add(__ldcg(p.partial + j));
+  const float top = warp_max(m);
+  s = warp_sum(top == -INFINITY ? s : s * gt_ex2(m - top));
+  z = warp_sum(z);
+  if (lane == 0) { zs[warp] = z; ms[warp] = make_float2(top, s); }
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  m = top;
+  for (int k = 1; k < WARPS; ++k) { z += zs[k]; add(ms[k]); }
+  const float loss = used ? logf(s) - (z - m * 0.6931471805599453f) : 0.0f;
+  if (f != p.ignore && !in_range) atomicExch(a.status, GT_ERR_INVALID_ARG);
+  p.s.stats[0] = make_float2(m, s);
+  p.s.ids[0] = used ? (int)f : LM_UNUSED;
+  p.s.q[0] = p.s.weight[0] = used ? 1.0f : 0.0f;
+  p.s.scalars->count = used ? 1 : 0;
+  if (p.row_loss) p.row_loss[0] = loss;
+  if (p.loss) *p.loss = loss;
+}
+
+template <int NC, bool VEC>
+__global__ void __launch_bounds__(THREADS) one_row_backward_kernel(const Rows a) {
+  gt_let_next_kernel_start();
+  gt_wait_for_previous_kernel();
+  const LmRows& p = a.r;
+  __shared__ float sums[WARPS][NC * 128];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const float l2 = 1.4426950408889634f / p.T;
+  const bool live = p.s.weight[0] != 0.0f;
+  const float c = live ? p.T * p.upstream[0] : 0.0f;            // one row: sum, mean and the row itself are the same
+  const float2 st = live ? p.s.stats[0] : make_float2(0.0f, 1.0f);
+  const float f = c / st.y;
+  Row<NC, VEC> x, dx;
+  dx.clear();
+  if (live) x.load(p.x, p.E); else x.clear();
+  const int first = p.s.ids[0];
+  auto word = [&](const Row<NC, VEC>& w, int v, float z) {
+    float g = live ? f * gt_ex2(z * l2 - st.x) : 0.0f;
+    if (v == first || (p.K > 1 && live)) {                      // the row's targets at this word
+      int lo = 0, hi = p.K;
+      while (lo < hi) { const int mid = (lo + hi) >> 1; if (p.s.ids[mid] < v) lo = mid + 1; else hi = mid; }
+      for (; lo < p.K && p.s.ids[lo] == v; ++lo) g -= c * p.s.q[lo];
+    }
+    float* to = p.dw + (long long)v * p.E;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int col = Row<NC, VEC>::column(i, 0);
+      float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (p.dw && p.acc_dw) {
+        if (VEC) {
+          if (col < p.E) *reinterpret_cast<float4*>(d) = *reinterpret_cast<const float4*>(to + col);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) if (Row<NC, VEC>::column(i, j) < p.E) d[j] = to[Row<NC, VEC>::column(i, j)];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        dx.v[i][j] = fmaf(g, w.v[i][j], dx.v[i][j]);
+        d[j] = fmaf(g, x.v[i][j], d[j]);
+      }
+      if (!p.dw) continue;
+      if (VEC) {
+        if (col < p.E) *reinterpret_cast<float4*>(to + col) = *reinterpret_cast<float4*>(d);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) if (Row<NC, VEC>::column(i, j) < p.E) to[Row<NC, VEC>::column(i, j)] = d[j];
+      }
+    }
+  };
+  const int stride = gridDim.x * WARPS;
+  for (int v = blockIdx.x * WARPS + warp; v < p.V; v += 2 * stride) {
+    const bool two = v + stride < p.V;
+    Row<NC, VEC> w0, w1;
+    w0.load(p.w + (long long)v * p.E, p.E);
+    w1.load(p.w + (long long)(two ? v + stride : v) * p.E, p.E);
+    const float z0 = warp_sum(x.dot(w0)), z1 = warp_sum(x.dot(w1));
+    word(w0, v, z0);
+    if (two) word(w1, v + stride, z1);
+  }
+  if (!p.dx_part) return;
+#pragma unroll
+  for (int i = 0; i < NC; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sums[warp][Row<NC, VEC>::column(i, j)] = dx.v[i][j];
+  __syncthreads();
+  for (int e = threadIdx.x; e < p.E; e += THREADS) {
+    float t = 0.0f;
+#pragma unroll
+    for (int k = 0; k < WARPS; ++k) t += sums[k][e];
+    p.dx_part[(long long)blockIdx.x * p.E + e] = t;
+  }
+}
+
 // dx (+)= the blocks' shares: 32 columns of a row per block, a warp takes every 32nd share, and the warps are added in order.
 __global__ void __launch_bounds__(1024) few_rows_dx_kernel(float* __restrict__ dx, const float* __restrict__ part, int parts, long long M, int E, int add) {
+  gt_let_next_kernel_start();
+  gt_wait_for_previous_kernel();
   __shared__ float sums[32][33];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int col = blockIdx.x * 32 + lane;
@@ -444,9 +583,18 @@ __global__ void __launch_bounds__(1024) few_rows_dx_kernel(float* __restrict__ d
 template <int MT, int C>
 int launch_as(gt_ctx* ctx, const Rows& a, bool backward) {
   const LmRows& p = a.r;
-  if (backward) few_rows_backward_kernel<MT, C><<<(unsigned)p.parts, THREADS, 0, ctx->stream>>>(a);
-  else few_rows_forward_kernel<MT, C><<<dim3((unsigned)p.parts, (unsigned)((p.M + MT - 1) / MT)), THREADS, 0, ctx->stream>>>(a);
-  GT_CUDA_OK(ctx, cudaGetLastError());
+  if (backward) GT_CUDA_OK(ctx, gt_launch_overlapped(few_rows_backward_kernel<MT, C>, dim3((unsigned)p.parts), dim3(THREADS), 0, ctx->stream, a));
+  else GT_CUDA_OK(ctx, gt_launch_overlapped(few_rows_forward_kernel<MT, C>, dim3((unsigned)p.parts, (unsigned)((p.M + MT - 1) / MT)), dim3(THREADS), 0, ctx->stream, a));
+  ctx->launches += 1;
+  return GT_OK;
+}
+template <int NC>
+int launch_one(gt_ctx* ctx, const Rows& a, bool backward) {
+  const LmRows& p = a.r;
+  const bool vec = p.E % 4 == 0 && (((uintptr_t)p.x | (uintptr_t)p.w | (uintptr_t)p.dw) & 15) == 0;
+  void (*kernel)(const Rows) = backward ? (vec ? one_row_backward_kernel<NC, true> : one_row_backward_kernel<NC, false>)
+                                        : (vec ? one_row_forward_kernel<NC, true> : one_row_forward_kernel<NC, false>);
+  GT_CUDA_OK(ctx, gt_launch_overlapped(kernel, dim3((unsigned)p.parts), dim3(THREADS), 0, ctx->stream, a));
   ctx->launches += 1;
   return GT_OK;
 }
@@ -465,7 +613,18 @@ int launch(gt_ctx* ctx, const LmRows& p, bool backward) {
   const int wide = (p.E + 127) / 128;
   a.r.cw = wide <= 1 ? 1 : wide <= 2 ? 2 : wide <= 4 ? 4 : 8;
   a.r.c = (p.E + 32 * a.r.cw - 1) / (32 * a.r.cw);
-  if (p.M == 1) return launch_for<1>(ctx, a, backward);
+  if (p.M == 1) {
+    switch ((p.E + 127) / 128) {
+      case 1: return launch_one<1>(ctx, a, backward);
+      case 2: return launch_one<2>(ctx, a, backward);
+      case 3: return launch_one<3>(ctx, a, backward);
+      case 4: return launch_one<4>(ctx, a, backward);
+      case 5: return launch_one<5>(ctx, a, backward);
+      case 6: return launch_one<6>(ctx, a, backward);
+      case 7: return launch_one<7>(ctx, a, backward);
+      default: return launch_one<8>(ctx, a, backward);
+    }
+  }
   if (p.M <= 4) return launch_for<4>(ctx, a, backward);
   return launch_for<16>(ctx, a, backward);
 }
@@ -480,8 +639,8 @@ bool gt_lm_few_rows(long long M, long long V, long long E) {
 }
 
 int gt_lm_rows_parts(gt_ctx* ctx, long long M, long long V, bool backward) {
-  const long long words = M == 1 ? 16 : 32, blocks = (V + words - 1) / words, tiles = M <= 16 ? 1 : (M + 15) / 16;
-  long long most = (M <= 1 ? 3ll : 2ll) * ctx->sm_count;         // blocks an SM; one row: 138 us with two, 130 with three, 137 with four
+  const long long words = M == 1 ? 2 * WARPS : WORDS, blocks = (V + words - 1) / words, tiles = M <= 16 ? 1 : (M + 15) / 16;
+  long long most = 2ll * ctx->sm_count;                          // blocks an SM; one row of 768 x 50257: 92, 92, 95, 97 us with 2, 3, 4, 6
   if (!backward) most = (most + tiles - 1) / tiles;
   return (int)(blocks < most ? blocks : most);
 }
@@ -491,8 +650,7 @@ int gt_lm_rows_forward(gt_ctx* ctx, const LmRows& p) { return launch(ctx, p, fal
 int gt_lm_rows_backward(gt_ctx* ctx, const LmRows& p, float* dx, int acc_dx) {
   int rc = launch(ctx, p, true);
   if (rc != GT_OK || !dx) return rc;
-  few_rows_dx_kernel<<<dim3((unsigned)((p.E + 31) / 32), (unsigned)p.M), 1024, 0, ctx->stream>>>(dx, p.dx_part, p.parts, p.M, p.E, acc_dx);
-  GT_CUDA_OK(ctx, cudaGetLastError());
+  GT_CUDA_OK(ctx, gt_launch_overlapped(few_rows_dx_kernel, dim3((unsigned)((p.E + 31) / 32), (unsigned)p.M), dim3(1024), 0, ctx->stream, dx, p.dx_part, p.parts, p.M, p.E, acc_dx));
   ctx->launches += 1;
   return GT_OK;
 }

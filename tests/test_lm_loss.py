@@ -171,7 +171,10 @@ def test_entry_points_refuse_bad_sizes(gt):
 # ---- values and gradients -------------------------------------------------------------------------
 
 SIZES = [(1, 1, 1), (1, 7, 3), (3, 2, 64), (2, 257, 65), (48, 500, 64), (129, 1000, 100), (300, 5003, 203), (257, 70001, 33), (520, 300, 768),
-         (64, 4096, 128), (1, 30011, 96), (17, 3001, 130)]
+         (64, 4096, 128), (1, 30011, 96), (17, 3001, 130),
+         # few rows: every number of columns a lane and of warps beside each other
+         (1, 2003, 768), (1, 900, 1024), (1, 515, 300), (1, 100, 600), (4, 1501, 700), (3, 333, 200), (2, 40, 1000), (16, 1200, 1000), (5, 700, 520),
+         (9, 401, 260), (64, 130, 900), (33, 290, 33)]
 
 
 @pytest.mark.gpu
