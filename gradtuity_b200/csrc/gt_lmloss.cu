@@ -490,8 +490,10 @@ Linear linear_layout(gt_ctx* ctx, void* saved, void* scratch, long long M, long 
   const long long tm = (M + LM_TILE - 1) / LM_TILE, te = (E + LM_TILE - 1) / LM_TILE, tv = (p.words + LM_TILE - 1) / LM_TILE;
   const long long ke = (E + LM_KBLOCK - 1) / LM_KBLOCK, kv = (p.words + LM_KBLOCK - 1) / LM_KBLOCK, km = (M + LM_KBLOCK - 1) / LM_KBLOCK;
   const long long pairs = ctx->sm_count / 2, step = tm * te * kv + tv * te * km + (l.pieces > 1 ? tm * tv * ke : 0);
-  const long long split = (3 * kv * pairs / 2 + step - 1) / step, most = (kv + 3) / 4;
-  p.dx_split = (int)(split < most ? split : most);
+  // Into units of a quarter of a pair's work, since it is not known how many rows count, and of 16 stages at least.
+  long long split = 3 * kv * pairs > 2 * step ? (4 * kv * pairs + step - 1) / step : 1;
+  if (split > kv / 16) split = kv / 16;
+  p.dx_split = (int)(split < 1 ? 1 : split);
 
   LmCarve c = {(char*)saved, 0};
   l.s = lm_saved(c, M, K);

@@ -134,6 +134,12 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b) {        // a i
 __device__ __forceinline__ float half_to_float(uint16_t h) { float f; asm("cvt.f32.f16 %0, %1;" : "=f"(f) : "h"(h)); return f; }
 __device__ __forceinline__ uint16_t float_to_half(float f) { uint16_t h; asm("cvt.rn.f16.f32 %0, %1;" : "=h"(h) : "f"(f)); return h; }
 
+// Adds without reading, so that nothing waits: one unit of a launch adds to an element, there is no order to depend on.
+__device__ __forceinline__ void add_to(float* p, float a) { asm volatile("red.global.add.f32 [%0], %1;" ::"l"(p), "f"(a) : "memory"); }
+__device__ __forceinline__ void add_to(float* p, const float4& a) {
+  asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(a.x), "f"(a.y), "f"(a.z), "f"(a.w) : "memory");
+}
+
 struct Maps {
   CUtensorMap x[2], w[2], g_mul[2], g_out[2];        // hi, lo
 };
@@ -402,22 +408,22 @@ __global__ void __launch_bounds__(THREADS, 1) lm_pair_kernel(const __grid_consta
         for (int c = 0; c < 4; ++c) {
           const int first = col0 + 32 * c;                      // within the piece
           if (first >= p.words_grad) break;
+#pragma unroll
+          for (int n = 32 * c; n < 32 * c + 32; n += 2) {       // in place: the halves of two columns take their registers
+            float g0 = fac.x * gt_ex2(fmaf(v[n], logit2, -st.x)), g1 = fac.x * gt_ex2(fmaf(v[n + 1], logit2, -st.x));
+            if (!live) { g0 = 0.0f; g1 = 0.0f; }
+            const uint32_t hi = pack_half2(g0, g1);
+            v[n] = __uint_as_float(hi);
+            v[n + 1] = __uint_as_float(pack_half2(g0 - half_to_float((uint16_t)hi), g1 - half_to_float((uint16_t)(hi >> 16))));
+          }
           if (lane == 0) tma_store_wait_read<0>();              // the staging tile is free again
           __syncwarp();
 #pragma unroll
           for (int j = 0; j < 4; ++j) {                         // 8 columns: 16 bytes of hi, 16 of lo
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int n = 32 * c + 8 * j + 2 * i;
-              float g0 = fac.x * gt_ex2(fmaf(v[n], logit2, -st.x)), g1 = fac.x * gt_ex2(fmaf(v[n + 1], logit2, -st.x));
-              if (!live) { g0 = 0.0f; g1 = 0.0f; }
-              hi[i] = pack_half2(g0, g1);
-              lo[i] = pack_half2(g0 - half_to_float((uint16_t)hi[i]), g1 - half_to_float((uint16_t)(hi[i] >> 16)));
-            }
             const int at = lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4);        // 64-byte swizzle
-            *reinterpret_cast<uint4*>(tile + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            *reinterpret_cast<uint4*>(tile + 2048 + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            const float* b = v + 32 * c + 8 * j;
+            *reinterpret_cast<float4*>(tile + at) = make_float4(b[0], b[2], b[4], b[6]);
+            *reinterpret_cast<float4*>(tile + 2048 + at) = make_float4(b[1], b[3], b[5], b[7]);
           }
           const int word0 = p.v0_grad + first;
           while (next_id < word0 + 32) {                        // this row's targets among these words
@@ -472,10 +478,10 @@ __global__ void __launch_bounds__(THREADS, 1) lm_pair_kernel(const __grid_consta
               const int r = it * 4 + (lane >> 3);
               const int to = __shfl_sync(0xffffffffu, mine, r);
               if (row_base + r < row_end && col < (int)p.E) {
-                float4 a = *reinterpret_cast<const float4*>(tile + r * 128 + ((j ^ (r & 7)) << 4));
-                float4* dst = reinterpret_cast<float4*>(out + (long long)to * p.E + col);
-                if (add) { const float4 b = *dst; a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w; }
-                *dst = a;
+                const float4 a = *reinterpret_cast<const float4*>(tile + r * 128 + ((j ^ (r & 7)) << 4));
+                float* dst = out + (long long)to * p.E + col;
+                if (add) add_to(dst, a);
+                else *reinterpret_cast<float4*>(dst) = a;
               }
             }
           } else {
@@ -483,9 +489,10 @@ __global__ void __launch_bounds__(THREADS, 1) lm_pair_kernel(const __grid_consta
             for (int r = 0; r < 32; ++r) {
               const int to = __shfl_sync(0xffffffffu, mine, r);
               if (row_base + r < row_end && first + lane < (int)p.E) {
-                float a = *reinterpret_cast<const float*>(tile + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+                const float a = *reinterpret_cast<const float*>(tile + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
                 float* dst = out + (long long)to * p.E + first + lane;
-                *dst = add ? *dst + a : a;
+                if (add) add_to(dst, a);
+                else *dst = a;
               }
             }
           }
