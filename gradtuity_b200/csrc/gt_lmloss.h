@@ -96,7 +96,7 @@ constexpr int LM_KBLOCK = 64;    // k elements of one stage
 inline bool lm_bad_sizes(long long M, long long V, long long K) {      // ids are float-encoded: exact below 2^24
   return M <= 0 || V <= 0 || K <= 0 || M > 0x7fffffff || V >= (1ll << 24) || K > LM_TOP_MAX;
 }
-inline bool lm_bad_temperature(float T) { return !(T > 0.0f) || T > 3.4e38f; }
+inline bool lm_bad_temperature(float T) { return !(T >= 1.0e-6f && T <= 1.0e6f); }      // T^2, 1 / T and their products stay finite
 inline bool lm_bad_reduction(int r) { return r != GT_REDUCE_NONE && r != GT_REDUCE_MEAN && r != GT_REDUCE_SUM; }
 
 // Sorted targets, weights and the count of the rows of a distillation (top_targets_kernel); also 0 for the loss of rows that do not count.

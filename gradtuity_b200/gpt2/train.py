@@ -71,11 +71,15 @@ def get_lr(step: int, warmup_steps: int, total_steps: int, base_lr: float) -> fl
 
 
 def train_step(model: GPT2Small, optimizer: AdamW, params: list, ids_t: Tensor, labels_t: Tensor, max_norm: float = 1.0,
-               world_size: int = 1) -> Tensor:
-    """One step in the reference's order; returns the loss tensor (still on the device)."""
-    logits = model(ids_t)
-    B, S, V = logits.shape
-    loss = logits.view((B * S, V)).cross_entropy(labels_t, reduction="mean")
+               world_size: int = 1, keep_logits: bool = True) -> Tensor:
+    """One step in the reference's order; returns the loss tensor (still on the device).  keep_logits=False takes the loss from the
+    hidden states in pieces of the vocabulary (GPT2Small.loss): no (B * S, V) logits, nor their gradient, in memory."""
+    if keep_logits:
+        logits = model(ids_t)
+        B, S, V = logits.shape
+        loss = logits.view((B * S, V)).cross_entropy(labels_t, reduction="mean")
+    else:
+        loss = model.loss(ids_t, labels_t)
     optimizer.zero_grad()
     loss.backward()
     if world_size > 1:
@@ -98,6 +102,7 @@ def main() -> None:
     ap.add_argument("--log_every", type=int, default=5)
     ap.add_argument("--n_layer", type=int, default=12)
     ap.add_argument("--vocab_size", type=int, default=50257)
+    ap.add_argument("--no_logits", action="store_true", help="loss and gradients of the LM head without keeping the logits")
     args = ap.parse_args()
 
     world = int(os.environ.get("WORLD_SIZE", "1"))
@@ -114,7 +119,8 @@ def main() -> None:
     t0 = None
     for step in range(args.steps):
         ids, labels = synthetic_batch(step, rank, args.batch_size, args.seq_len, args.vocab_size)
-        loss = train_step(model, opt, params, Tensor.from_numpy(ids), Tensor.from_numpy(labels), args.max_norm, world)
+        loss = train_step(model, opt, params, Tensor.from_numpy(ids), Tensor.from_numpy(labels), args.max_norm, world,
+                          keep_logits=not args.no_logits)
         if step == 2:
             _lib.device_status()
             t0 = time.perf_counter()

@@ -1205,8 +1205,8 @@ class Tensor:
     def _loss_checks(opname: str, reduction: str, temperature: float = 1.0) -> int:
         if reduction not in _lib.REDUCTIONS:
             raise ValueError(f"{opname} reduction must be 'none', 'mean' or 'sum', got {reduction!r}")
-        if not (temperature > 0.0 and math.isfinite(temperature)):
-            raise ValueError(f"{opname} temperature must be positive and finite, got {temperature}")
+        if not 1e-6 <= temperature <= 1e6:
+            raise ValueError(f"{opname} temperature must be between 1e-6 and 1e6, got {temperature}")
         return _lib.REDUCTIONS[reduction]
 
     @staticmethod
@@ -1244,10 +1244,15 @@ class Tensor:
 
         def _backward(g: "Tensor") -> None:
             dx, acc_dx = grad_target(x) if x.requires_grad else (None, False)
-            dw, acc_dw = grad_target(weight) if weight.requires_grad else (None, False)
+            # one tensor as input and weight: dx and dw are computed side by side, so the second cannot go to the same buffer
+            twin = alloc_storage(V * E * F32) if weight is x and x.requires_grad else None
+            dw, acc_dw = (twin.ptr, False) if twin is not None else grad_target(weight) if weight.requires_grad else (None, False)
             scratch = None if keep else alloc_storage(n_scratch)
             _call("gt_linear_loss_backward", dx, dw, saved.ptr, work or scratch.ptr, x.ptr, weight.ptr, g.ptr, M, V, E, top, temperature, reduction,
                   prec, acc_dx, acc_dw)
+            if twin is not None:
+                _call("gt_scale", dx, twin.ptr, 1.0, V * E, 1)
+                twin.free()
             if scratch is not None:
                 scratch.free()
 

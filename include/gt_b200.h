@@ -392,7 +392,7 @@ int gt_cross_entropy_backward(gt_ctx* ctx, float* dlogits, int64_t ld_dlogits, c
  * Sparse targets: row t has (id, q) pairs.  Cross entropy has one pair with q = 1 (none where targets[t] == ignore_index).
  * Distillation takes the teacher's top logits: ids and teacher are (M, K), K <= 1024, in any order, an id may repeat; an entry
  * is in use when its id is >= 0 and its logit is above -inf (a NaN logit is not in use); q = softmax(teacher / T) over the
- * entries in use.  A row with no target in use has no loss and no gradient and does not count.  With z = logits / T,
+ * entries in use, 1e-6 <= T <= 1e6.  A row with no target in use has no loss and no gradient and does not count.  With z = logits / T,
  *     loss_t = T^2 sum_k q_tk (log q_tk - log softmax(z_t)[id_tk]),   d loss_t / d logits_t = T (softmax(z_t) - q_t)
  * loss receives M values (GT_REDUCE_NONE) or one: their sum, or their mean over the rows that count (0 when none does).
  * ids are float-encoded (V < 2^24); one that is in use and >= V, or a target outside [0, V) other than ignore_index, sets the

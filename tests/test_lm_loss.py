@@ -131,6 +131,8 @@ def fake(*shape):
     (lambda: fake(4, 2, 2).topk_distillation(fake(4, 2), fake(4, 2)), "expects 2D logits"),
     (lambda: fake(4, 9).topk_distillation(fake(4, 2), fake(4, 2), temperature=float("inf")), "temperature must be"),
     (lambda: fake(4, 9).topk_distillation(fake(4, 2), fake(4, 2), temperature=float("nan")), "temperature must be"),
+    (lambda: fake(4, 9).topk_distillation(fake(4, 2), fake(4, 2), temperature=1e-7), "temperature must be"),
+    (lambda: fake(4, 9).topk_distillation(fake(4, 2), fake(4, 2), temperature=-2.0), "temperature must be"),
     (lambda: fake(4, 9).topk_distillation(fake(3, 2), fake(3, 2)), "batch size mismatch"),
     (lambda: fake(4, 9).topk_distillation(fake(4, 2), fake(4, 2), reduction="avg"), "reduction must be"),
 ])
@@ -174,7 +176,9 @@ SIZES = [(1, 1, 1), (1, 7, 3), (3, 2, 64), (2, 257, 65), (48, 500, 64), (129, 10
          (64, 4096, 128), (1, 30011, 96), (17, 3001, 130),
          # few rows: every number of columns a lane and of warps beside each other
          (1, 2003, 768), (1, 900, 1024), (1, 515, 300), (1, 100, 600), (4, 1501, 700), (3, 333, 200), (2, 40, 1000), (16, 1200, 1000), (5, 700, 520),
-         (9, 401, 260), (64, 130, 900), (33, 290, 33)]
+         (9, 401, 260), (64, 130, 900), (33, 290, 33),
+         # two pieces of the vocabulary, the second ragged, and dx in shares
+         (1100, 33001, 40)]
 
 
 @pytest.mark.gpu
@@ -427,6 +431,98 @@ def test_losses_in_flight_do_not_share_memory(gt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("M, V, E", [(4, 9000, 96), (60, 2000, 200), (300, 30001, 100), (1100, 33001, 40), (700, 5000, 513)])
+def test_repeats_are_equal_to_the_bit(gt, M, V, E):
+    """Units of work are handed out as they come, sums are taken in a fixed order: the same call gives the same bits."""
+    rng = np.random.default_rng([M, V])
+    x, w = hidden(rng, M, V, E)
+    ids, teacher = teacher_of(rng, M, V, 9)
+    ti, tt = Tensor.from_numpy(ids), Tensor.from_numpy(teacher)
+    runs = [run_linear(x, w, lambda a, b: a.linear_topk_distillation(b, ti, tt, temperature=2.0, precision="3xtf32")) for _ in range(4)]
+    for run in runs[1:]:
+        assert all(np.array_equal(a, b) for a, b in zip(run, runs[0]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M, V, E", [(8192, 12800, 64), (2500, 40000, 130)])
+def test_many_pieces_against_the_path_through_the_logits(gt, monkeypatch, M, V, E):
+    """Several pieces of the vocabulary, dx of each added to the last: against linear_tied and cross_entropy, whose products are
+    3xTF32 (5e-6 off); a third of the rows is left out."""
+    monkeypatch.setenv("GRADTUITY_GEMM_PRECISION", "3xtf32")
+    rng = np.random.default_rng(21)
+    x, w = hidden(rng, M, V, E)
+    targets = rng.integers(0, V, M).astype(np.float32)
+    out = rng.random(M) < 0.33
+    labels = np.where(out, -100, targets).astype(np.float32)
+    loss, dx, dw = run_linear(x, w, lambda a, b: a.linear_cross_entropy(b, Tensor.from_numpy(labels)))
+    xt, wt = Tensor.from_numpy(x[~out], requires_grad=True), Tensor.from_numpy(w, requires_grad=True)
+    want = xt.linear_tied(wt).cross_entropy(Tensor.from_numpy(targets[~out]))
+    assert loss[0] == pytest.approx(want.item(), rel=1e-5)
+    want.backward()
+    assert not dx[out].any()
+    assert rel(dx[~out], xt.grad.numpy().astype(np.float64)) < 2e-5 and rel(dw, wt.grad.numpy().astype(np.float64)) < 2e-5
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M, V, E", [(1, 700, 64), (12, 700, 64), (150, 1200, 72)])
+def test_rows_left_out_hold_garbage(gt, M, V, E):
+    """Padding rows of NaN and infinities: no trace in the loss or dw, dx 0 there, or what it was when gradients accumulate."""
+    rng = np.random.default_rng([22, M])
+    x, w = hidden(rng, M, V, E)
+    targets = rng.integers(0, V, M).astype(np.float32)
+    out = rng.random(M) < 0.5
+    out[0] = True
+    targets[out] = -1
+    logits = np.where(out[:, None], 0.0, x.astype(np.float64)) @ w.astype(np.float64).T
+    want, g = oracle(logits, *hard(M, V, targets, -1), np.zeros(M), 1.0, "mean")
+    x[out] = np.where(rng.random((int(out.sum()), E)) < 0.5, np.nan, np.inf)
+    xt, wt = Tensor.from_numpy(x, requires_grad=True), Tensor.from_numpy(w, requires_grad=True)
+    for times in (1, 2):
+        loss = xt.linear_cross_entropy(wt, Tensor.from_numpy(targets), ignore_index=-1, precision="3xtf32")
+        assert abs(loss.item() - want) < 1e-5
+        loss.backward()
+        clean = np.where(out[:, None], 0.0, x)
+        dx = xt.grad.numpy()
+        assert not dx[out].any()
+        assert rel(dx, times * (g @ w)) < 1e-5 and rel(wt.grad.numpy(), times * (g.T @ clean)) < 1e-5
+    assert _lib.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V, E", [(30, 24), (300, 70)])
+def test_one_tensor_as_input_and_weight(gt, V, E):
+    rng = np.random.default_rng(23)
+    w = (rng.standard_normal((V, E)) / np.sqrt(E)).astype(np.float32)
+    targets = rng.integers(0, V, V).astype(np.float32)
+    _, g = oracle(w.astype(np.float64) @ w.astype(np.float64).T, *hard(V, V, targets), np.zeros(V), 1.0, "mean")
+    wt = Tensor.from_numpy(w, requires_grad=True)
+    wt.linear_cross_entropy(wt, Tensor.from_numpy(targets), precision="3xtf32").backward()
+    assert rel(wt.grad.numpy(), g @ w + g.T @ w) < 1e-5
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("first", ["cross_entropy", "distillation"])
+@pytest.mark.parametrize("B, C", [(40, 30001), (9, 500)])
+def test_two_losses_of_the_same_logits(gt, first, B, C):
+    """Both prepare the logits' gradient in their forward pass; one is taken over, the other added."""
+    rng = np.random.default_rng(24)
+    z = (rng.standard_normal((B, C)) * 2).astype(np.float32)
+    targets = rng.integers(0, C, B).astype(np.float32)
+    ids, teacher = teacher_of(rng, B, C, 6)
+    q, counted = dense_targets(B, C, ids, teacher, 2.0)
+    a, ga = oracle(z.astype(np.float64), *hard(B, C, targets), np.zeros(B), 1.0, "mean")
+    b, gb = oracle(z.astype(np.float64), q, counted, entropy_of(B, ids, teacher, 2.0), 2.0, "mean")
+    zt = Tensor.from_numpy(z, requires_grad=True)
+    losses = [zt.cross_entropy(Tensor.from_numpy(targets)), zt.topk_distillation(Tensor.from_numpy(ids), Tensor.from_numpy(teacher), temperature=2.0)]
+    if first == "distillation":
+        losses.reverse()
+    total = losses[0].add(losses[1])
+    assert total.item() == pytest.approx(a + b, rel=1e-5)
+    total.backward()
+    assert rel(zt.grad.numpy(), ga + gb) < 1e-5
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("op", ["linear_cross_entropy", "linear_topk_distillation", "topk_distillation"])
 def test_gradients_against_differences(gt, op):
     """Central differences of the 32-bit loss along random directions: a loss of about 5 is exact to 5 2^-22, which the
@@ -530,3 +626,25 @@ def test_gpt2_trained_with_both_losses(gt, monkeypatch):
     assert _lib.device_status() == 0
     assert all(np.isfinite(p.numpy()).all() for p in params)
     assert any((p.numpy() != b).any() for p, b in zip(params, before))
+
+
+@pytest.mark.gpu
+def test_train_step_without_logits(gt, monkeypatch):
+    """The training step's option gives the step's loss and the same updated parameters, up to the products' rounding."""
+    from gradtuity_b200.gpt2.train import build_model, synthetic_batch, train_step
+    from gradtuity_b200.optim import AdamW
+
+    monkeypatch.setenv("GRADTUITY_GEMM_PRECISION", "3xtf32")
+    ids, labels = synthetic_batch(0, 0, 2, 32, 301)
+    losses, grads = [], []
+    for keep in (True, False):
+        model = build_model(vocab_size=301, seq_len=32, n_embd=64, n_layer=1, n_head=1)
+        params = model.parameters()
+        loss = train_step(model, AdamW(params, lr=1e-3), params, Tensor.from_numpy(ids), Tensor.from_numpy(labels), keep_logits=keep)
+        assert _lib.device_status() == 0
+        losses.append(loss.item())
+        grads.append([p.grad.numpy() for p in params])
+    assert losses[0] == pytest.approx(losses[1], abs=1e-5)
+    largest = max(np.linalg.norm(g) for g in grads[0])
+    for a, b in zip(*grads):
+        assert np.linalg.norm(a - b) < 5e-5 * max(np.linalg.norm(a), 1e-3 * largest)
