@@ -7,7 +7,7 @@
 // by fp16 tensor-core instructions, which run at twice the rate of tf32 and read half the bytes.  With products == 1 only hi hi'
 // is taken: the operand rounding of tf32.
 // The tensor cores add into their 32-bit accumulators by cutting off, not rounding (measured: a sum of K = 512 terms of one
-// sign comes out 1.5e-6 too small).  So no accumulator stays there for long: after three stages (192 of K) the
+// sign comes out 1.5e-6 too small).  So no accumulator stays there for long: after two or three stages (128 or 192 of K) the
 // epilogue warps add it to their registers, rounding to nearest, while the next one fills the other half of tensor memory.
 //
 // Work.  One kernel, persistent, a pair of CTAs (cta_group::2) per 256 x 256 tile, handed out by a counter: the units of a launch
@@ -50,7 +50,7 @@ struct Params {
   float* dx_partial;
   long long E;
   int M, V, K;
-  int products, sub_stages;
+  int products, sub_z, sub_mul;   // stages between two roundings to nearest: of the logits, of dx and dW
   int forward;                    // 1: STATS units over all words, nothing else
   int words_grad, v0_grad;        // piece of the G units (0 words: none)
   int words_mul, v0_mul;          // piece of the dx and dW units (0: none)
@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(THREADS, 1) lm_pair_kernel(const __grid_consta
           if (!mbar_wait_cluster(bar_tempty + 8 * acc, aph ^ 1u, abort_flag, p.status)) { ok = false; break; }
           tc_fence_after();
           const uint32_t d_tmem = tmem_base + (uint32_t)(acc * TILE);
-          const int end = min(t.kb_hi, kb + p.sub_stages);
+          const int end = min(t.kb_hi, kb + (t.kind <= GRAD ? p.sub_z : p.sub_mul));
           uint32_t started = 0;
           for (; kb < end; ++kb) {
             if (!mbar_wait_cluster(bar_full + 8 * s, ph, abort_flag, p.status)) { ok = false; break; }
@@ -355,7 +355,8 @@ __global__ void __launch_bounds__(THREADS, 1) lm_pair_kernel(const __grid_consta
 #pragma unroll
         for (int i = 0; i < 128; ++i) v[i] = 0.0f;
       }
-      for (int kb = t.kb_lo; kb < t.kb_hi; kb += p.sub_stages) {
+      const int sub = t.kind <= GRAD ? p.sub_z : p.sub_mul;
+      for (int kb = t.kb_lo; kb < t.kb_hi; kb += sub) {
         const bool got = mbar_wait_cluster(bar_tfull + 8 * acc, aph, abort_flag, p.status);
         if (!__all_sync(0xffffffffu, got)) { ok = false; break; }
         tc_fence_after();
@@ -557,11 +558,13 @@ Params common_params(gt_ctx* ctx, const LmProblem& p) {
   a.partial = p.partial;
   a.E = p.E; a.M = (int)p.M; a.V = (int)p.V;
   a.products = p.products;
-  // Between two roundings to nearest: 192 of K with three products (36 additions), 512 with one, whose operands are rounded to 11
-  // bits anyway.  Every hand-over costs the tensor cores about 450 cycles.  8192 x 768 x 50257 with gradients, by stages of 64
-  // between two hand-overs, time and error of dx against 64 bits: 2: 6.91 ms, 3.0e-7; 3: 6.46 ms, 4.3e-7; 4: 6.46 ms,
-  // 5.8e-7; 6: 6.31 ms, 8.6e-7.
-  a.sub_stages = p.products == 3 ? 3 : 8;
+  // Between two roundings to nearest: 128 or 192 of K with three products (24, 36 additions), 512 with one, whose operands are rounded
+  // to 11 bits anyway.  Every hand-over costs the tensor cores about 450 cycles.  8192 x 768 x 50257 with gradients, by stages of
+  // 64 between two hand-overs, time and error of dx against 64 bits: 2: 6.91 ms, 3.0e-7; 3: 6.46 ms, 4.3e-7; 4: 6.46 ms,
+  // 5.8e-7; 6: 6.31 ms, 8.6e-7.  The logits have the smaller number: the loss subtracts the targets' from them in 32 bits, so
+  // their bias stays in it.  It is the same one forward and backward: p is a quotient of the two, and the bias cancels.
+  a.sub_z = p.products == 3 ? 2 : 8;
+  a.sub_mul = p.products == 3 ? 3 : 8;
   a.dx_split = 1;
   return a;
 }
@@ -607,9 +610,6 @@ int gt_lm_stats(gt_ctx* ctx, const LmProblem& p) {
   if (rc != GT_OK) return rc;
   Params a = common_params(ctx, p);
   a.forward = 1;
-  // The loss subtracts logits of the targets in 32 bits from these: their bias stays in it, so it is kept smaller (losses of 1024 rows
-  // of 768 x 50257 off by 1.8e-7 with two stages, 2.8e-7 with three, for 4 % more time).
-  if (p.products == 3) a.sub_stages = 2;
   a.counter = p.counters;
   return launch(ctx, maps, a, tiles(p.M) * tiles(p.V));
 }
