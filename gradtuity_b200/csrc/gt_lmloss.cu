@@ -340,25 +340,40 @@ __global__ void __launch_bounds__(256) target_loss_kernel(float* __restrict__ ro
     const float log_s = logf(st.y), top = st.x * 0.6931471805599453f;
     const float* xr = x + t * E;
     const bool vec = ((uintptr_t)x & 15) == 0 && ((uintptr_t)w & 15) == 0 && E % 4 == 0;
-    for (int k = warp % WARPS_A_ROW; k < K; k += WARPS_A_ROW) {
-      const int id = s.ids[t * K + k];
-      if (id == LM_UNUSED) break;
-      const float q = s.q[t * K + k];
-      if (q == 0.0f) continue;
-      const float* wr = w + (long long)id * E;
-      float z = 0.0f;
+    constexpr int AT_ONCE = WARPS_A_ROW > 1 ? 4 : 1;          // targets whose words are read together
+    for (int k0 = warp % WARPS_A_ROW * AT_ONCE; k0 < K; k0 += WARPS_A_ROW * AT_ONCE) {
+      const float* wr[AT_ONCE];
+      float q[AT_ONCE], z[AT_ONCE];
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; ++k) {
+        const int id = k0 + k < K ? s.ids[t * K + k0 + k] : LM_UNUSED;
+        q[k] = id != LM_UNUSED ? s.q[t * K + k0 + k] : 0.0f;
+        wr[k] = w + (long long)(id != LM_UNUSED ? id : 0) * E;
+        z[k] = 0.0f;
+      }
       if (vec) {
-#pragma unroll 4
+#pragma unroll 2
         for (int e = 4 * l; e < E; e += 128) {
-          const float4 a = *reinterpret_cast<const float4*>(xr + e), b = *reinterpret_cast<const float4*>(wr + e);
-          z = fmaf(a.x, b.x, z); z = fmaf(a.y, b.y, z); z = fmaf(a.z, b.z, z); z = fmaf(a.w, b.w, z);
+          const float4 a = *reinterpret_cast<const float4*>(xr + e);
+#pragma unroll
+          for (int k = 0; k < AT_ONCE; ++k) {
+            const float4 b = *reinterpret_cast<const float4*>(wr[k] + e);
+            z[k] = fmaf(a.x, b.x, z[k]); z[k] = fmaf(a.y, b.y, z[k]); z[k] = fmaf(a.z, b.z, z[k]); z[k] = fmaf(a.w, b.w, z[k]);
+          }
         }
       } else {
 #pragma unroll 4
-        for (int e = l; e < E; e += 32) z = fmaf(xr[e], wr[e], z);
+        for (int e = l; e < E; e += 32) {
+          const float a = xr[e];
+#pragma unroll
+          for (int k = 0; k < AT_ONCE; ++k) z[k] = fmaf(a, wr[k][e], z[k]);
+        }
       }
-      z = warp_sum(z) / T;
-      cross += q * ((z - top) - log_s);
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; ++k) {
+        const float sum = warp_sum(z[k]) / T;
+        if (q[k] != 0.0f) cross += q[k] * ((sum - top) - log_s);
+      }
     }
   }
   if (WARPS_A_ROW > 1) {
@@ -431,18 +446,19 @@ __global__ void __launch_bounds__(1024) begin_backward_kernel(const float* __res
   }
 }
 
-// dx (+)= the shares of a piece, in order.
-__global__ void __launch_bounds__(256) add_shares_kernel(float* __restrict__ dx, const float* __restrict__ shares, int n_shares, long long M, long long E,
-                                                         int add, LmSaved s) {
+// to (+)= the shares of a piece, in order: (n_shares, M, E).  A block per row; dx: the rows that count, elsewhere all M.
+__global__ void __launch_bounds__(256) add_shares_kernel(float* __restrict__ to, const float* __restrict__ shares, int n_shares, long long M, long long E,
+                                                         int add, const int* __restrict__ row_of, const int* __restrict__ count) {
   gt_let_next_kernel_start();
   gt_wait_for_previous_kernel();
   const long long i = blockIdx.x;
-  if (i >= s.scalars->count) return;
-  float* to = dx + (long long)s.row_of[i] * E;
+  if (count && i >= *count) return;
+  float* out = to + (row_of ? (long long)row_of[i] : i) * E;
   for (long long e = threadIdx.x; e < E; e += 256) {
-    float a = add ? to[e] : 0.0f;
+    float a = add ? out[e] : 0.0f;
+#pragma unroll 4
     for (int j = 0; j < n_shares; ++j) a += shares[((long long)j * M + i) * E + e];
-    to[e] = a;
+    out[e] = a;
   }
 }
 
@@ -485,15 +501,13 @@ Linear linear_layout(gt_ctx* ctx, void* saved, void* scratch, long long M, long 
   if (p.words > V) p.words = V;
   p.pitch_v = (p.words + 7) / 8 * 8;
   l.pieces = (int)((V + p.words - 1) / p.words);
-  // A dx tile runs over all words of a piece.  Where that is long against what a pair of CTAs has to do in the whole step (few rows:
-  // few tiles, large pieces), its words are shared out, and the shares added up afterwards.
-  const long long tm = (M + LM_TILE - 1) / LM_TILE, te = (E + LM_TILE - 1) / LM_TILE, tv = (p.words + LM_TILE - 1) / LM_TILE;
-  const long long ke = (E + LM_KBLOCK - 1) / LM_KBLOCK, kv = (p.words + LM_KBLOCK - 1) / LM_KBLOCK, km = (M + LM_KBLOCK - 1) / LM_KBLOCK;
-  const long long pairs = ctx->sm_count / 2, step = tm * te * kv + tv * te * km + (l.pieces > 1 ? tm * tv * ke : 0);
-  // Into units of a quarter of a pair's work, since it is not known how many rows count, and of 16 stages at least.
-  long long split = 3 * kv * pairs > 2 * step ? (4 * kv * pairs + step - 1) / step : 1;
-  if (split > kv / 16) split = kv / 16;
-  p.dx_split = (int)(split < 1 ? 1 : split);
+  p.dx_split = lm_shares((p.words + LM_KBLOCK - 1) / LM_KBLOCK, lm_step_stages(p, p.words, l.pieces > 1 ? p.words : 0), ctx->sm_count / 2);
+  // dW's shares, step by step: the most that a step needs (full pieces beside a full one, beside the last one; the last one alone)
+  long long dw_rows = 0;
+  for (long long piece = l.pieces > 3 ? l.pieces - 3 : 0; piece < l.pieces; ++piece) {
+    const long long n = lm_dw_split(ctx, p, lm_piece_words(p, piece), lm_piece_words(p, piece + 1)) * lm_piece_words(p, piece);
+    if (n > lm_piece_words(p, piece) && n > dw_rows) dw_rows = n;
+  }
 
   LmCarve c = {(char*)saved, 0};
   l.s = lm_saved(c, M, K);
@@ -512,6 +526,7 @@ Linear linear_layout(gt_ctx* ctx, void* saved, void* scratch, long long M, long 
     if (p.products == 3) p.g[i].lo = b.take<uint16_t>(M * p.pitch_v);
   }
   if (p.dx_split > 1) p.dx_partial = b.take<float>(p.dx_split * M * E);
+  if (dw_rows > 0) p.dw_partial = b.take<float>(dw_rows * E);
   l.scratch_bytes = f.at > b.at ? f.at : b.at;
   p.scalars = l.s.scalars; p.row_of = l.s.row_of; p.stats = l.s.stats; p.factor = l.s.factor; p.ids = l.s.ids; p.q = l.s.q;
   return l;
@@ -644,8 +659,16 @@ extern "C" int gt_linear_loss_backward(gt_ctx* ctx, float* dx, float* dw, void* 
     int rc = gt_lm_step(ctx, p, piece);
     if (rc != GT_OK) return rc;
     if (piece > 0 && dx && p.dx_split > 1) {
-      GT_CUDA_OK(ctx, gt_launch_overlapped(add_shares_kernel, dim3((unsigned)M), dim3(256), 0, ctx->stream, dx, p.dx_partial, p.dx_split, M, E, acc_dx || piece > 1, l.s));
-          ctx->launches += 1;
+      GT_CUDA_OK(ctx, gt_launch_overlapped(add_shares_kernel, dim3((unsigned)M), dim3(256), 0, ctx->stream, dx, p.dx_partial, p.dx_split, M, E, acc_dx || piece > 1,
+                                           l.s.row_of, &l.s.scalars->count));
+      ctx->launches += 1;
+    }
+    const long long words = lm_piece_words(p, piece - 1);
+    const int dw_split = lm_dw_split(ctx, p, words, lm_piece_words(p, piece));
+    if (dw && dw_split > 1) {
+      GT_CUDA_OK(ctx, gt_launch_overlapped(add_shares_kernel, dim3((unsigned)words), dim3(256), 0, ctx->stream, dw + (long long)(piece - 1) * p.words * E, p.dw_partial,
+                                           dw_split, words, E, acc_dw, (const int*)nullptr, (const int*)nullptr));
+      ctx->launches += 1;
     }
   }
   return GT_OK;

@@ -86,7 +86,8 @@ struct LmProblem {
   const float2* factor;          // G = factor.x e^(z - m) - factor.y q, by compact row
   const int* ids; const float* q; int K;
   float* dx; float* dw; int acc_dx, acc_dw;
-  float* dx_partial; int dx_split;   // dx of a piece in `dx_split` shares of its words, when that is over 1
+  float* dx_partial; int dx_split;   // dx of a piece in `dx_split` shares of its words, when that is over 1: (dx_split, M, E)
+  float* dw_partial;                 // dW of a piece in lm_dw_split shares of the rows, when that is over 1: (shares, words of the piece, E)
   int* counters;                 // one zeroed int per launch: the next unit of work
 };
 
@@ -102,6 +103,28 @@ inline bool lm_bad_reduction(int r) { return r != GT_REDUCE_NONE && r != GT_REDU
 // Sorted targets, weights and the count of the rows of a distillation (top_targets_kernel); also 0 for the loss of rows that do not count.
 int gt_lm_top_targets(gt_ctx* ctx, const LmSaved& s, float* row_loss, const float* ids, const float* teacher, long long M, long long V, long long K,
                       float T);
+
+// The sums of a step: what a pair of CTAs has to do in it, in stages, times `pairs`.
+inline long long lm_step_stages(const LmProblem& p, long long words_mul, long long words_grad) {
+  auto tiles = [](long long n) { return (n + LM_TILE - 1) / LM_TILE; };
+  auto stages = [](long long n) { return (n + LM_KBLOCK - 1) / LM_KBLOCK; };
+  return tiles(p.M) * tiles(p.E) * stages(words_mul) + tiles(words_mul) * tiles(p.E) * stages(p.M) + tiles(p.M) * tiles(words_grad) * stages(p.E);
+}
+// A dx (dW) tile runs over all words of a piece (all rows).  Where these `k` stages are long against a pair's part of the step, they are
+// shared out and the shares added up afterwards: into units of a quarter of a pair's part, since it is not known how many rows
+// count, and of 16 stages at least.
+inline int lm_shares(long long k, long long step, long long pairs) {
+  long long n = 3 * k * pairs > 2 * step ? (4 * k * pairs + step - 1) / step : 1;
+  if (n > k / 16) n = k / 16;
+  return (int)(n < 1 ? 1 : n);
+}
+inline int lm_dw_split(gt_ctx* ctx, const LmProblem& p, long long words_mul, long long words_grad) {
+  return words_mul ? lm_shares((p.M + LM_KBLOCK - 1) / LM_KBLOCK, lm_step_stages(p, words_mul, words_grad), ctx->sm_count / 2) : 1;
+}
+inline long long lm_piece_words(const LmProblem& p, long long piece) {
+  const long long v0 = piece * p.words;
+  return v0 < 0 || v0 >= p.V ? 0 : p.V - v0 < p.words ? p.V - v0 : p.words;
+}
 
 // Forward: per row and half tile of words, (maximum, sum of exponentials).
 int gt_lm_stats(gt_ctx* ctx, const LmProblem& p);

@@ -47,14 +47,14 @@ struct Params {
   const float* q;
   float2* partial;
   float* dx; float* dw;
-  float* dx_partial;
+  float* dx_partial; float* dw_partial;
   long long E;
   int M, V, K;
   int products, sub_z, sub_mul;   // stages between two roundings to nearest: of the logits, of dx and dW
   int forward;                    // 1: STATS units over all words, nothing else
   int words_grad, v0_grad;        // piece of the G units (0 words: none)
   int words_mul, v0_mul;          // piece of the dx and dW units (0: none)
-  int dx_split, acc_dx, acc_dw, want_dx, want_dw;
+  int dx_split, dw_split, acc_dx, acc_dw, want_dx, want_dw;
   int vec_dx, vec_dw;
 };
 
@@ -62,7 +62,7 @@ struct Unit {
   int kind;
   int m0, n0;                     // tile origin
   int kb_lo, kb_hi;               // stages
-  int share;                      // of a dx tile
+  int share;                      // of a dx or dW tile
 };
 
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
@@ -72,10 +72,12 @@ __device__ __forceinline__ bool unit_of(const Params& p, int rows, int u, Unit& 
   const int tiles_m = ceil_div(rows, TILE), tiles_e = ceil_div((int)p.E, TILE);
   t.share = 0;
   if (p.want_dw && p.words_mul) {
-    const int n = ceil_div(p.words_mul, TILE) * tiles_e;
+    const int n = ceil_div(p.words_mul, TILE) * tiles_e * p.dw_split;
     if (u < n) {
-      t.kind = DW; t.m0 = u / tiles_e * TILE; t.n0 = u % tiles_e * TILE;
-      t.kb_lo = 0; t.kb_hi = ceil_div(rows, BK);
+      const int kb = ceil_div(rows, BK), per = ceil_div(kb, p.dw_split);
+      t.kind = DW; t.share = u % p.dw_split; u /= p.dw_split;
+      t.m0 = u / tiles_e * TILE; t.n0 = u % tiles_e * TILE;
+      t.kb_lo = min(kb, t.share * per); t.kb_hi = min(kb, t.kb_lo + per);
       return true;
     }
     u -= n;
@@ -453,12 +455,13 @@ __global__ void __launch_bounds__(THREADS, 1) lm_pair_kernel(const __grid_consta
         // dx or dW: 32 x 32 blocks through shared memory, so that a warp writes whole lines
         const bool is_dw = t.kind == DW;
         const float alpha = is_dw ? p.scalars->dw : p.scalars->dx;
-        const bool share = !is_dw && p.dx_split > 1;
+        const bool share = (is_dw ? p.dw_split : p.dx_split) > 1;
         const bool add = share ? false : is_dw ? p.acc_dw != 0 : (p.acc_dx != 0 || p.v0_mul > 0);
-        const bool vec = is_dw ? p.vec_dw != 0 : (share || p.vec_dx != 0) && p.E % 4 == 0;
+        const bool vec = (share || (is_dw ? p.vec_dw : p.vec_dx) != 0) && p.E % 4 == 0;
         const int row_base = t.m0 + (int)rank * HALF + quarter * 32;
         const int row_end = is_dw ? p.words_mul : rows;
-        float* out = is_dw ? p.dw + (long long)p.v0_mul * p.E : share ? p.dx_partial + (long long)t.share * p.M * p.E : p.dx;
+        float* out = is_dw ? (share ? p.dw_partial + (long long)t.share * p.words_mul * p.E : p.dw + (long long)p.v0_mul * p.E)
+                           : (share ? p.dx_partial + (long long)t.share * p.M * p.E : p.dx);
         int mine = row_base + lane;                             // lane l knows where row l goes
         if (!is_dw && !share && mine < row_end) mine = p.row_of[mine];
         if (lane == 0) tma_store_wait_read<0>();                // a G unit may have used the staging tile before
@@ -565,7 +568,7 @@ Params common_params(gt_ctx* ctx, const LmProblem& p) {
   // their bias stays in it.  It is the same one forward and backward: p is a quotient of the two, and the bias cancels.
   a.sub_z = p.products == 3 ? 2 : 8;
   a.sub_mul = p.products == 3 ? 3 : 8;
-  a.dx_split = 1;
+  a.dx_split = a.dw_split = 1;
   return a;
 }
 
@@ -618,10 +621,8 @@ int gt_lm_step(gt_ctx* ctx, const LmProblem& p, int piece) {
   Maps maps;
   memset(&maps, 0, sizeof(maps));
   Params a = common_params(ctx, p);
-  auto words_of = [&](long long v0) { return (int)(v0 < 0 || v0 >= p.V ? 0 : p.V - v0 < p.words ? p.V - v0 : p.words); };
-  const long long v_grad = (long long)piece * p.words, v_mul = v_grad - p.words;
-  a.words_grad = words_of(v_grad); a.v0_grad = (int)v_grad;
-  a.words_mul = words_of(v_mul); a.v0_mul = (int)v_mul;
+a.words_grad = (int)lm_piece_words(p, piece); a.v0_grad = (int)(piece * p.words);
+  a.words_mul = (int)lm_piece_words(p, piece - 1); a.v0_mul = (int)((piece - 1) * p.words);
   int rc = encode_pair(ctx, maps.x, p.x, p, p.E, p.M, p.pitch_e, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc == GT_OK) rc = encode_pair(ctx, maps.w, p.w, p, p.E, p.V, p.pitch_e, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B);
   if (rc == GT_OK && a.words_mul)
@@ -633,9 +634,10 @@ int gt_lm_step(gt_ctx* ctx, const LmProblem& p, int piece) {
   a.dx = p.dx; a.dw = p.dw; a.acc_dx = p.acc_dx; a.acc_dw = p.acc_dw;
   a.want_dx = p.dx != nullptr; a.want_dw = p.dw != nullptr;
   a.dx_split = p.dx_split; a.dx_partial = p.dx_partial;
+  a.dw_split = lm_dw_split(ctx, p, a.words_mul, a.words_grad); a.dw_partial = p.dw_partial;
   a.vec_dx = ((uintptr_t)p.dx & 15) == 0 && p.E % 4 == 0;
   a.vec_dw = ((uintptr_t)p.dw & 15) == 0 && p.E % 4 == 0;
-  const long long units = tiles(a.words_mul) * tiles(p.E) * (p.dw != nullptr) +
+  const long long units = tiles(a.words_mul) * tiles(p.E) * a.dw_split * (p.dw != nullptr) +
                           (a.words_mul ? tiles(p.M) * tiles(p.E) * p.dx_split * (p.dx != nullptr) : 0) + tiles(p.M) * tiles(a.words_grad);
   return launch(ctx, maps, a, units);
 }
