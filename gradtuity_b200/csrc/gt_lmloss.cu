@@ -266,25 +266,44 @@ __global__ void __launch_bounds__(256) split_kernel(const float* __restrict__ x,
 
 // ---- rows ------------------------------------------------------------------------------------------
 
-// The linear forms: (m, s) of the rows that count from the parts' (tiles of words, or blocks).  32 rows a block, their parts shared
-// out over 32 warps, so that a warp reads whole lines.
-__global__ void __launch_bounds__(1024) join_stats_kernel(const float2* __restrict__ partial, int parts, long long M, LmSaved s) {
+// The rows' losses added up by one block, in 64 bits and in a fixed order.
+template <int THREADS>
+__device__ __forceinline__ void sum_losses(float* loss, const float* row_loss, long long M, int count, int mean) {
+  __shared__ double sums[THREADS / 32];
+  double a = 0.0;
+  for (long long r = threadIdx.x; r < M; r += THREADS) a += __ldcg(row_loss + r);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = a;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int k = 1; k < THREADS / 32; ++k) a += sums[k];
+    if (mean && count > 0) a /= (double)count;
+    *loss = (float)a;
+  }
+}
+
+// After the products: (m, s) of the rows that count from their tiles', and their losses from the targets' logits.  32 rows a block, the
+// tiles shared out over 32 warps, so that a warp reads whole lines; then a warp per row.  The last block to end adds the losses up.
+__global__ void __launch_bounds__(1024) join_tiles_kernel(const float2* __restrict__ partial, int parts, const float* __restrict__ target_z,
+                                                          float* __restrict__ row_loss, float* __restrict__ loss, long long M, int K, float T, int mean,
+                                                          LmSaved s, unsigned long long* ticket) {
   gt_let_next_kernel_start();
   gt_wait_for_previous_kernel();
   __shared__ float2 red[32][33];
-  const int w = threadIdx.x >> 5, l = threadIdx.x & 31;
+  __shared__ int last;
+  const int w = threadIdx.x >> 5, l = threadIdx.x & 31, count = s.scalars->count;
   const long long i = (long long)blockIdx.x * 32 + l;
-  const bool live = i < s.scalars->count;
   float m = -INFINITY, sum = 0.0f;                            // m in units of log 2
-  auto add = [&](float2 b) {
-    const float top = fmaxf(m, b.x);
-    if (top == -INFINITY) { sum += b.y; return; }             // nothing but words that do not exist; or a NaN, which counts
-    sum = sum * gt_ex2(m - top) + b.y * gt_ex2(b.x - top);
-    m = top;
-  };
-  if (live) {
+  if (i < count) {
 #pragma unroll 4
-    for (int j = w; j < parts; j += 32) add(partial[(long long)j * M + i]);
+    for (int j = w; j < parts; j += 32) {
+      const float2 b = partial[(long long)j * M + i];
+      const float top = fmaxf(m, b.x);
+      if (top == -INFINITY) { sum += b.y; continue; }         // nothing but words that do not exist; or a NaN, which counts
+      sum = sum * gt_ex2(m - top) + b.y * gt_ex2(b.x - top);
+      m = top;
+    }
   }
   red[w][l] = make_float2(m, sum);
   __syncthreads();
@@ -293,55 +312,67 @@ __global__ void __launch_bounds__(1024) join_stats_kernel(const float2* __restri
   const float top = warp_max(mine.x);
   sum = warp_sum(top == -INFINITY ? mine.y : mine.y * gt_ex2(mine.x - top));
   const long long r = (long long)blockIdx.x * 32 + w;
-  if (l == 0 && r < s.scalars->count) s.stats[r] = make_float2(top, sum);
+  if (r < count) {
+    const long long t = s.row_of[r];
+    const float log_s = logf(sum);
+    float cross = 0.0f;
+    for (int k = l; k < K; k += 32) {
+      if (s.ids[t * K + k] == LM_UNUSED) break;
+      const float q = s.q[t * K + k];
+      if (q != 0.0f) cross += q * ((target_z[r * K + k] - top) * 0.6931471805599453f - log_s);
+    }
+    cross = warp_sum(cross);
+    if (l == 0) {
+      s.stats[r] = make_float2(top, sum);
+      row_loss[t] = T * T * (s.konst[t] - cross);
+    }
+  }
+  if (!loss) return;
+  __threadfence();
+  __syncthreads();
+  unsigned none;
+  if (threadIdx.x == 0) last = lm_count_out(ticket, gridDim.x, 0, &none);
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  sum_losses<1024>(loss, row_loss, M, count, mean);
 }
 
-// Losses of the rows, from the logits of their targets, taken in 32 bits straight from x and w.  WARPS_A_ROW warps share a row's targets.
-// The rows are the compact ones, with their statistics there; or, with `partial`, all rows, whose parts' statistics are by row
-// and are joined here (WARPS_A_ROW = 8).  The last block to end adds the rows' losses up, in 64 bits and in a fixed order.
-template <int WARPS_A_ROW>
-__global__ void __launch_bounds__(256) target_loss_kernel(float* __restrict__ row_loss, float* __restrict__ loss, const float* __restrict__ x,
+// After the few rows' products (distillation): the same, a block per row; the parts are blocks' and by row, and the targets' logits are
+// taken straight from x and w.
+__global__ void __launch_bounds__(256) join_blocks_kernel(float* __restrict__ row_loss, float* __restrict__ loss, const float* __restrict__ x,
                                                           const float* __restrict__ w, long long M, int E, int K, float T, int mean,
                                                           const float2* __restrict__ partial, int parts, LmSaved s, unsigned long long* ticket) {
   gt_let_next_kernel_start();
   gt_wait_for_previous_kernel();
   __shared__ float part[8];
   __shared__ float2 joined[8];
-  __shared__ double sums[8];
   __shared__ int last;
   const int warp = threadIdx.x >> 5, l = threadIdx.x & 31;
-  const long long i = (long long)blockIdx.x * (8 / WARPS_A_ROW) + warp / WARPS_A_ROW;
-  const bool live = partial ? s.weight[i] != 0.0f : i < s.scalars->count;
-  long long t = 0;
+  const long long t = blockIdx.x;
+  float m = -INFINITY, sum = 0.0f;
+  auto add = [&](float2 b) {
+    const float top = fmaxf(m, b.x);
+    if (top == -INFINITY) { sum += b.y; return; }
+    sum = sum * gt_ex2(m - top) + b.y * gt_ex2(b.x - top);
+    m = top;
+  };
+  for (int j = threadIdx.x; j < parts; j += 256) add(partial[(long long)j * M + t]);
+  const float warp_top = warp_max(m);
+  sum = warp_sum(warp_top == -INFINITY ? sum : sum * gt_ex2(m - warp_top));
+  if (l == 0) joined[warp] = make_float2(warp_top, sum);
+  __syncthreads();
+  m = -INFINITY; sum = 0.0f;
+  for (int k = 0; k < 8; ++k) add(joined[k]);
+  if (threadIdx.x == 0) s.stats[t] = make_float2(m, sum);
+  const bool live = s.weight[t] != 0.0f;
   float cross = 0.0f;
-  float2 st = make_float2(0.0f, 1.0f);
-  if (WARPS_A_ROW == 8 && partial) {
-    float m = -INFINITY, sum = 0.0f;
-    auto add = [&](float2 b) {
-      const float top = fmaxf(m, b.x);
-      if (top == -INFINITY) { sum += b.y; return; }
-      sum = sum * gt_ex2(m - top) + b.y * gt_ex2(b.x - top);
-      m = top;
-    };
-    for (int j = threadIdx.x; j < parts; j += 256) add(partial[(long long)j * M + i]);
-    const float top = warp_max(m);
-    sum = warp_sum(top == -INFINITY ? sum : sum * gt_ex2(m - top));
-    if (l == 0) joined[warp] = make_float2(top, sum);
-    __syncthreads();
-    m = -INFINITY; sum = 0.0f;
-    for (int k = 0; k < 8; ++k) add(joined[k]);
-    st = make_float2(m, sum);
-    if (threadIdx.x == 0) s.stats[i] = st;
-  } else if (live) {
-    st = s.stats[i];
-  }
   if (live) {
-    t = partial ? i : s.row_of[i];
-    const float log_s = logf(st.y), top = st.x * 0.6931471805599453f;
+    const float log_s = logf(sum), top = m * 0.6931471805599453f;
     const float* xr = x + t * E;
     const bool vec = ((uintptr_t)x & 15) == 0 && ((uintptr_t)w & 15) == 0 && E % 4 == 0;
-    constexpr int AT_ONCE = WARPS_A_ROW > 1 ? 4 : 1;          // targets whose words are read together
-    for (int k0 = warp % WARPS_A_ROW * AT_ONCE; k0 < K; k0 += WARPS_A_ROW * AT_ONCE) {
+    constexpr int AT_ONCE = 4;                                // targets whose words are read together
+    for (int k0 = warp * AT_ONCE; k0 < K; k0 += 8 * AT_ONCE) {
       const float* wr[AT_ONCE];
       float q[AT_ONCE], z[AT_ONCE];
 #pragma unroll
@@ -376,13 +407,11 @@ __global__ void __launch_bounds__(256) target_loss_kernel(float* __restrict__ ro
       }
     }
   }
-  if (WARPS_A_ROW > 1) {
-    if (l == 0) part[warp] = cross;
-    __syncthreads();
-    cross = 0.0f;
-    for (int k = 0; k < WARPS_A_ROW; ++k) cross += part[warp / WARPS_A_ROW * WARPS_A_ROW + k];
-  }
-  if (live && l == 0 && warp % WARPS_A_ROW == 0) row_loss[t] = T * T * (s.konst[t] - cross);
+  if (l == 0) part[warp] = cross;
+  __syncthreads();
+  cross = 0.0f;
+  for (int k = 0; k < 8; ++k) cross += part[k];
+  if (live && threadIdx.x == 0) row_loss[t] = T * T * (s.konst[t] - cross);
   if (!loss) return;
   __threadfence();
   __syncthreads();
@@ -391,17 +420,7 @@ __global__ void __launch_bounds__(256) target_loss_kernel(float* __restrict__ ro
   __syncthreads();
   if (!last) return;
   __threadfence();
-  double a = 0.0;
-  for (long long r = threadIdx.x; r < M; r += 256) a += __ldcg(row_loss + r);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
-  if (l == 0) sums[warp] = a;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int k = 1; k < 8; ++k) a += sums[k];
-    if (mean && s.scalars->count > 0) a /= (double)s.scalars->count;
-    *loss = (float)a;
-  }
+  sum_losses<256>(loss, row_loss, M, s.scalars->count, mean);
 }
 
 // Before the backward walk.  Block 0: what the rows' gradients are multiplied by.  The halves of G hold 2^14 u (p - q), u = 1, or with
@@ -521,6 +540,7 @@ Linear linear_layout(gt_ctx* ctx, void* saved, void* scratch, long long M, long 
   LmCarve b = f;
   l.row_loss = f.take<float>(M);
   p.partial = f.take<float2>((V + LM_TILE - 1) / LM_TILE * 2 * M);
+  p.target_z = f.take<float>(M * K);
   for (int i = 0; i < (l.pieces > 1 ? 2 : 1); ++i) {
     p.g[i].hi = b.take<uint16_t>(M * p.pitch_v);
     if (p.products == 3) p.g[i].lo = b.take<uint16_t>(M * p.pitch_v);
@@ -553,30 +573,13 @@ int prepare_linear(gt_ctx* ctx, const LmSaved& s, int* counters, float* row_loss
   return GT_OK;
 }
 
-int finish_rows(gt_ctx* ctx, float* row_loss, float* loss, const float2* partial, int parts, const float* x, const float* w, long long M,
-                long long E, long long K, float T, int reduction, bool by_row, const LmSaved& s) {
-  float* out = reduction == GT_REDUCE_NONE ? nullptr : loss;
-  const int mean = reduction == GT_REDUCE_MEAN;
-  if (by_row) {
-    GT_CUDA_OK(ctx, gt_launch_overlapped(target_loss_kernel<8>, dim3((unsigned)M), dim3(256), 0, ctx->stream, row_loss, out, x, w, M, (int)E, (int)K, T, mean,
-                                         partial, parts, s, lm_ticket(ctx)));
-    ctx->launches += 1;
-    return GT_OK;
-  }
-  GT_CUDA_OK(ctx, gt_launch_overlapped(join_stats_kernel, dim3((unsigned)((M + 31) / 32)), dim3(1024), 0, ctx->stream, partial, parts, M, s));
-  void (*kernel)(float*, float*, const float*, const float*, long long, int, int, float, int, const float2*, int, LmSaved, unsigned long long*) =
-      K == 1 ? target_loss_kernel<1> : target_loss_kernel<8>;
-  GT_CUDA_OK(ctx, gt_launch_overlapped(kernel, dim3((unsigned)(K == 1 ? (M + 7) / 8 : M)), dim3(256), 0, ctx->stream, row_loss, out, x, w, M, (int)E, (int)K, T, mean,
-                                       (const float2*)nullptr, 0, s, lm_ticket(ctx)));
-  ctx->launches += 2;
-  return GT_OK;
-}
-
 int linear_forward(gt_ctx* ctx, float* loss, void* saved, void* scratch, const float* x, const float* w, const float* targets, float ignore,
                    const float* ids, const float* teacher, int64_t M, int64_t V, int64_t E, int64_t K, float T, int reduction, int precision) {
   const Linear l = linear_layout(ctx, saved, scratch, M, V, E, K, precision);
   const LmSaved& s = l.s;
   float* rows = reduction == GT_REDUCE_NONE ? loss : l.row_loss;
+  float* sum = reduction == GT_REDUCE_NONE ? nullptr : loss;
+  const int mean = reduction == GT_REDUCE_MEAN;
   if (l.few_rows) {
     LmRows r = rows_problem(l, x, w, M, V, E, K, T, reduction);
     r.parts = gt_lm_rows_parts(ctx, M, V, false);
@@ -584,11 +587,15 @@ int linear_forward(gt_ctx* ctx, float* loss, void* saved, void* scratch, const f
     if (!targets) {
       int rc = gt_lm_top_targets(ctx, s, rows, ids, teacher, M, V, K, T);
       if (rc == GT_OK) rc = gt_lm_rows_forward(ctx, r);
-      return rc != GT_OK ? rc : finish_rows(ctx, rows, loss, l.p.partial, r.parts, x, w, M, E, K, T, reduction, true, s);
+      if (rc != GT_OK) return rc;
+      GT_CUDA_OK(ctx, gt_launch_overlapped(join_blocks_kernel, dim3((unsigned)M), dim3(256), 0, ctx->stream, rows, sum, x, w, M, (int)E, (int)K, T, mean, l.p.partial,
+                                           r.parts, s, lm_ticket(ctx)));
+      ctx->launches += 1;
+      return GT_OK;
     }
     r.targets = targets; r.ignore = ignore;
     r.row_loss = rows;
-    r.loss = reduction == GT_REDUCE_NONE ? nullptr : loss;
+    r.loss = sum;
     return gt_lm_rows_forward(ctx, r);
   }
   int rc = prepare_linear(ctx, s, l.p.counters, rows, targets, ignore, ids, teacher, M, V, K, T);
@@ -601,7 +608,10 @@ int linear_forward(gt_ctx* ctx, float* loss, void* saved, void* scratch, const f
   ctx->launches += 2;
   rc = gt_lm_stats(ctx, l.p);
   if (rc != GT_OK) return rc;
-  return finish_rows(ctx, rows, loss, l.p.partial, (int)((V + LM_TILE - 1) / LM_TILE * 2), x, w, M, E, K, T, reduction, false, s);
+  GT_CUDA_OK(ctx, gt_launch_overlapped(join_tiles_kernel, dim3((unsigned)((M + 31) / 32)), dim3(1024), 0, ctx->stream, l.p.partial,
+                                       (int)((V + LM_TILE - 1) / LM_TILE * 2), l.p.target_z, rows, sum, M, (int)K, T, mean, s, lm_ticket(ctx)));
+  ctx->launches += 1;
+  return GT_OK;
 }
 
 }  // namespace

@@ -82,6 +82,7 @@ struct LmProblem {
   const int* row_of;             // compact row -> row of x
   LmSplit x, w, g[2];
   float2* partial;               // (V tiles x 2, M) maxima and sums of the forward pass
+  float* target_z;               // forward: z log2(e) of the targets, (M, K) by compact row
   const float2* stats;           // (m log2(e), s) by compact row
   const float2* factor;          // G = factor.x e^(z - m) - factor.y q, by compact row
   const int* ids; const float* q; int K;
@@ -126,7 +127,7 @@ inline long long lm_piece_words(const LmProblem& p, long long piece) {
   return v0 < 0 || v0 >= p.V ? 0 : p.V - v0 < p.words ? p.V - v0 : p.words;
 }
 
-// Forward: per row and half tile of words, (maximum, sum of exponentials).
+// Forward: per row and half tile of words, (maximum, sum of exponentials); and the targets' logits.
 int gt_lm_stats(gt_ctx* ctx, const LmProblem& p);
 // One step of the backward walk over the pieces: G of piece `piece` (if it exists), and dx, dw of the piece before.
 int gt_lm_step(gt_ctx* ctx, const LmProblem& p, int piece);

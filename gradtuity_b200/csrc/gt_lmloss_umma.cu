@@ -46,6 +46,7 @@ struct Params {
   const int* ids;
   const float* q;
   float2* partial;
+  float* target_z;
   float* dx; float* dw;
   float* dx_partial; float* dw_partial;
   long long E;
@@ -342,11 +343,11 @@ __global__ void __launch_bounds__(THREADS, 1) lm_pair_kernel(const __grid_consta
       float2 st = make_float2(0.0f, 1.0f), fac = make_float2(0.0f, 0.0f);
       const int* ids = nullptr; const float* q = nullptr;
       int k = 0, next_id = 0x7fffffff;
-      if (t.kind == GRAD && row < rows) {
-        st = p.stats[row]; fac = p.factor[row];
+      if (t.kind <= GRAD && row < rows) {
+        if (t.kind == GRAD) { st = p.stats[row]; fac = p.factor[row]; }
         const long long r = p.row_of[row];
         ids = p.ids + r * p.K; q = p.q + r * p.K;
-        const int first = p.v0_grad + col0;                     // first target at or behind this warp's columns
+        const int first = (t.kind == GRAD ? p.v0_grad : 0) + col0;                     // first target at or behind this warp's columns
         int lo = 0, hi = p.K;
         while (lo < hi) { const int mid = (lo + hi) >> 1; if (ids[mid] < first) lo = mid + 1; else hi = mid; }
         k = lo;
@@ -386,6 +387,24 @@ __global__ void __launch_bounds__(THREADS, 1) lm_pair_kernel(const __grid_consta
 
       if (t.kind == STATS) {
         const int left = p.V - col0;                            // columns of this half that are words
+        // The targets among these words: a lane puts its row through the staging tile (its own part of it, swizzled) to pick from
+        // it by index.  The loss takes the targets' logits from here rather than from an exact product: what the additions in
+        // tensor memory cut off is then in both sides of z - log sum e^z.
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int word0 = col0 + 32 * c;
+          if (!__any_sync(0xffffffffu, next_id < word0 + 32)) continue;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<float4*>(tile + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+                make_float4(v[32 * c + 4 * j], v[32 * c + 4 * j + 1], v[32 * c + 4 * j + 2], v[32 * c + 4 * j + 3]);
+          while (next_id < word0 + 32) {
+            const int n = next_id - word0;
+            p.target_z[(long long)row * p.K + k] = logit2 * *reinterpret_cast<const float*>(tile + lane * 128 + (((n >> 2) ^ (lane & 7)) << 4) + (n & 3) * 4);
+            next_id = ++k < p.K ? ids[k] : 0x7fffffff;
+          }
+          __syncwarp();
+        }
         float2 out = make_float2(-INFINITY, 0.0f);
         if (left > 0) {
           if (left < HALF) {
@@ -558,7 +577,7 @@ Params common_params(gt_ctx* ctx, const LmProblem& p) {
   memset(&a, 0, sizeof(a));
   a.scalars = p.scalars; a.status = ctx->d_status; a.row_of = p.row_of;
   a.stats = p.stats; a.factor = p.factor; a.ids = p.ids; a.q = p.q; a.K = p.K;
-  a.partial = p.partial;
+  a.partial = p.partial; a.target_z = p.target_z;
   a.E = p.E; a.M = (int)p.M; a.V = (int)p.V;
   a.products = p.products;
   // Between two roundings to nearest: 128 or 192 of K with three products (24, 36 additions), 512 with one, whose operands are rounded
