@@ -465,23 +465,23 @@ __global__ void __launch_bounds__(1024) begin_backward_kernel(const float* __res
   }
 }
 
-// to (+)= the shares of a piece, in order: (n_shares, M, E).  A block per row; dx: the rows that count, elsewhere all M.
+// to (+)= the shares of a piece, in order: (n_shares, M, E).  A block per row and 256 columns; dx: the rows that count, elsewhere all M.
 __global__ void __launch_bounds__(256) add_shares_kernel(float* __restrict__ to, const float* __restrict__ shares, int n_shares, long long M, long long E,
                                                          int add, const int* __restrict__ row_of, const int* __restrict__ count) {
   gt_let_next_kernel_start();
   gt_wait_for_previous_kernel();
   const long long i = blockIdx.x;
   if (count && i >= *count) return;
-  float* out = to + (row_of ? (long long)row_of[i] : i) * E;
-  for (long long e = threadIdx.x; e < E; e += 256) {
-    float a = add ? out[e] : 0.0f;
-#pragma unroll 4
-    for (int j = 0; j < n_shares; ++j) a += shares[((long long)j * M + i) * E + e];
-    out[e] = a;
-  }
+  const long long e = (long long)blockIdx.y * 256 + threadIdx.x;
+  if (e >= E) return;
+  float* out = to + (row_of ? (long long)row_of[i] : i) * E + e;
+  float a = add ? *out : 0.0f;
+#pragma unroll 8
+  for (int j = 0; j < n_shares; ++j) a += shares[((long long)j * M + i) * E + e];
+  *out = a;
 }
 
-bool bad_width(long long E) { return E <= 0 || E > (1 << 24); }
+bool bad_width(long long E) { return E <= 0 || E >= (1 << 24); }
 
 bool bad_precision(int p) { return p != GT_PREC_TF32 && p != GT_PREC_TF32X3 && p != GT_PREC_FP32; }
 
@@ -669,14 +669,14 @@ extern "C" int gt_linear_loss_backward(gt_ctx* ctx, float* dx, float* dw, void* 
     int rc = gt_lm_step(ctx, p, piece);
     if (rc != GT_OK) return rc;
     if (piece > 0 && dx && p.dx_split > 1) {
-      GT_CUDA_OK(ctx, gt_launch_overlapped(add_shares_kernel, dim3((unsigned)M), dim3(256), 0, ctx->stream, dx, p.dx_partial, p.dx_split, M, E, acc_dx || piece > 1,
+      GT_CUDA_OK(ctx, gt_launch_overlapped(add_shares_kernel, dim3((unsigned)M, (unsigned)((E + 255) / 256)), dim3(256), 0, ctx->stream, dx, p.dx_partial, p.dx_split, M, E, acc_dx || piece > 1,
                                            l.s.row_of, &l.s.scalars->count));
       ctx->launches += 1;
     }
     const long long words = lm_piece_words(p, piece - 1);
     const int dw_split = lm_dw_split(ctx, p, words, lm_piece_words(p, piece));
     if (dw && dw_split > 1) {
-      GT_CUDA_OK(ctx, gt_launch_overlapped(add_shares_kernel, dim3((unsigned)words), dim3(256), 0, ctx->stream, dw + (long long)(piece - 1) * p.words * E, p.dw_partial,
+      GT_CUDA_OK(ctx, gt_launch_overlapped(add_shares_kernel, dim3((unsigned)words, (unsigned)((E + 255) / 256)), dim3(256), 0, ctx->stream, dw + (long long)(piece - 1) * p.words * E, p.dw_partial,
                                            dw_split, words, E, acc_dw, (const int*)nullptr, (const int*)nullptr));
       ctx->launches += 1;
     }

@@ -143,6 +143,12 @@ __device__ __forceinline__ void add_to(float* p, const float4& a) {
   asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p), "f"(a.x), "f"(a.y), "f"(a.z), "f"(a.w) : "memory");
 }
 
+// Arrival that passes on no data of this thread's.  (A releasing one of cluster scope first waits for the thread's stores to global
+// memory; an epilogue warp has a whole tile of them on their way.)
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
 struct Maps {
   CUtensorMap x[2], w[2], g_mul[2], g_out[2];        // hi, lo
 };
@@ -198,9 +204,13 @@ __global__ void __launch_bounds__(THREADS, 1) lm_pair_kernel(const __grid_consta
   auto take_unit = [&](bool whole_warp, int& u) -> bool {
     const bool got = mbar_wait_cluster(bar_sfull + 8 * slot, slot_ph, abort_flag, p.status);
     if (whole_warp ? !__all_sync(0xffffffffu, got) : !got) return false;
-    u = slots[slot];
-    if (whole_warp) __syncwarp();
-    if (!whole_warp || lane == 0) mbar_arrive_cluster(leader_sempty + 8 * slot);
+    if (whole_warp) {
+      u = __shfl_sync(0xffffffffu, lane == 0 ? slots[slot] : 0, 0);       // lane 0 has read the slot when it hands it back
+      if (lane == 0) mbar_arrive_cluster_relaxed(leader_sempty + 8 * slot);
+    } else {
+      u = slots[slot];
+      mbar_arrive_cluster(leader_sempty + 8 * slot);
+    }
     if (++slot == SLOTS) { slot = 0; slot_ph ^= 1u; }
     return true;
   };
@@ -380,7 +390,7 @@ __global__ void __launch_bounds__(THREADS, 1) lm_pair_kernel(const __grid_consta
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(leader_tempty + 8 * acc);
+        if (lane == 0) mbar_arrive_cluster_relaxed(leader_tempty + 8 * acc);      // the loads are complete (wait::ld)
         if (++acc == 2) { acc = 0; aph ^= 1u; }
       }
       if (!ok) break;
