@@ -353,6 +353,8 @@ __global__ void __launch_bounds__(THREADS, 1) lm_pair_kernel(const __grid_consta
       float2 st = make_float2(0.0f, 1.0f), fac = make_float2(0.0f, 0.0f);
       const int* ids = nullptr; const float* q = nullptr;
       int k = 0, next_id = 0x7fffffff;
+      if (t.kind == DX) st.x = p.scalars->dx;
+      if (t.kind == DW) st.x = p.scalars->dw;
       if (t.kind <= GRAD && row < rows) {
         if (t.kind == GRAD) { st = p.stats[row]; fac = p.factor[row]; }
         const long long r = p.row_of[row];
@@ -483,7 +485,7 @@ __global__ void __launch_bounds__(THREADS, 1) lm_pair_kernel(const __grid_consta
       } else {
         // dx or dW: 32 x 32 blocks through shared memory, so that a warp writes whole lines
         const bool is_dw = t.kind == DW;
-        const float alpha = is_dw ? p.scalars->dw : p.scalars->dx;
+        const float alpha = st.x;
         const bool share = (is_dw ? p.dw_split : p.dx_split) > 1;
         const bool add = share ? false : is_dw ? p.acc_dw != 0 : (p.acc_dx != 0 || p.v0_mul > 0);
         const bool vec = (share || (is_dw ? p.vec_dw : p.vec_dx) != 0) && p.E % 4 == 0;
@@ -491,6 +493,9 @@ __global__ void __launch_bounds__(THREADS, 1) lm_pair_kernel(const __grid_consta
         const int row_end = is_dw ? p.words_mul : rows;
         float* out = is_dw ? (share ? p.dw_partial + (long long)t.share * p.words_mul * p.E : p.dw + (long long)p.v0_mul * p.E)
                            : (share ? p.dx_partial + (long long)t.share * p.M * p.E : p.dx);
+        const bool linear = is_dw || share;
+        float* const line = out + (long long)(row_base + (lane >> 3)) * p.E + 4 * (lane & 7);
+        const int lines = row_end - row_base - (lane >> 3);
         int mine = row_base + lane;                             // lane l knows where row l goes
         if (!is_dw && !share && mine < row_end) mine = p.row_of[mine];
         if (lane == 0) tma_store_wait_read<0>();                // a G unit may have used the staging tile before
@@ -504,7 +509,19 @@ __global__ void __launch_bounds__(THREADS, 1) lm_pair_kernel(const __grid_consta
             *reinterpret_cast<float4*>(tile + lane * 128 + ((j ^ (lane & 7)) << 4)) =
                 make_float4(alpha * v[32 * c + 4 * j], alpha * v[32 * c + 4 * j + 1], alpha * v[32 * c + 4 * j + 2], alpha * v[32 * c + 4 * j + 3]);
           __syncwarp();
-          if (vec) {
+          if (vec && linear) {                                  // rows one after the other: a pointer that moves on
+            float* dst = line + first;
+            const bool inside = first + 4 * (lane & 7) < (int)p.E;
+#pragma unroll
+            for (int it = 0; it < 8; ++it, dst += 4 * p.E) {
+              const int r = it * 4 + (lane >> 3);
+              if (inside && 4 * it < lines) {
+                const float4 a = *reinterpret_cast<const float4*>(tile + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+                if (add) add_to(dst, a);
+                else *reinterpret_cast<float4*>(dst) = a;
+              }
+            }
+          } else if (vec) {
             const int j = lane & 7, col = first + 4 * j;
 #pragma unroll
             for (int it = 0; it < 8; ++it) {
