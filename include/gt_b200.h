@@ -400,7 +400,8 @@ int gt_cross_entropy_backward(gt_ctx* ctx, float* dlogits, int64_t ld_dlogits, c
  *
  * The linear forms take hidden states x and the vocabulary matrix w; the logits are x w^T, computed in pieces of the
  * vocabulary and never kept.  precision: GT_PREC_TF32 rounds the operands of the products to 11 bits; GT_PREC_TF32X3 and
- * GT_PREC_FP32 are as exact as sums in 32 bits.  `saved` is what the forward pass leaves for the backward pass, `scratch` is free
+ * GT_PREC_FP32 are as exact as sums in 32 bits, which a few rows (up to 16, or 64 with little work) get in any precision.  w must
+ * not change between the two calls.  dx and dw must not overlap.  `saved` is what the forward pass leaves for the backward pass, `scratch` is free
  * for other use once the call's work is done; gt_linear_loss_sizes gives the bytes of both (256-byte aligned, both not NULL;
  * K = 1 for cross entropy).  gt_linear_loss_backward serves both losses: T = 1, K = 1 for cross entropy; the other arguments as
  * in the forward call.  upstream: the gradient of the loss, on the device: M values for GT_REDUCE_NONE, else one.  dx or dw

@@ -251,10 +251,10 @@ def test_topk_distillation(gt, B, C, K, T, reduction, duplicates):
 @pytest.mark.gpu
 @pytest.mark.parametrize("op", ["linear_cross_entropy", "linear_topk_distillation", "topk_distillation"])
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
-def test_rows_that_do_not_count(gt, op, reduction):
+@pytest.mark.parametrize("M, V, E", [(33, 300, 40), (1, 300, 40), (200, 4500, 40), (1500, 300, 300)])
+def test_rows_that_do_not_count(gt, op, reduction, M, V, E):
     """All rows without a target: loss 0 and gradients that are written, as zeros; masked places may hold anything."""
     rng = np.random.default_rng(5)
-    M, V, E = 33, 300, 40
     x, w = hidden(rng, M, V, E)
     xt, wt = Tensor.from_numpy(x, requires_grad=True), Tensor.from_numpy(w, requires_grad=True)
     ids = np.full((M, 4), -1, np.float32)
@@ -267,6 +267,7 @@ def test_rows_that_do_not_count(gt, op, reduction):
     elif op == "linear_topk_distillation":
         loss = xt.linear_topk_distillation(wt, ti, tt, reduction=reduction)
     else:
+        xt = Tensor.from_numpy(rng.standard_normal((M, V)).astype(np.float32), requires_grad=True)
         loss = xt.topk_distillation(ti, tt, reduction=reduction)
     assert not loss.numpy().any()
     (loss.sum() if reduction == "none" else loss).backward()
