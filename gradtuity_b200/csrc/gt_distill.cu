@@ -411,7 +411,7 @@ extern "C" int gt_topk_distillation(gt_ctx* ctx, float* loss, void* saved, float
   int rc = gt_lm_top_targets(ctx, p.s, p.row_loss, ids, teacher, B, C, K, temperature);
   if (rc != GT_OK) return rc;
   // The row in shared memory: with a gradient, for rows long enough to be worth a block of 1024 threads and short enough to fit
-  // (54 000 words beside the targets), where logits and gradient lie alike with respect to 16 bytes.
+  // (53248 words beside the targets), where logits and gradient lie alike with respect to 16 bytes.
   if (dlogits && C >= ROW_MIN_C && C <= ROW_MAX_C && K <= ROW_MAX_TOP && (((uintptr_t)logits ^ (uintptr_t)dlogits) & 15) == 0 &&
       (ld_logits - ld_dlogits) % 4 == 0 && ((uintptr_t)logits & 3) == 0) {
     GT_SMEM_OPT_IN(ctx, distill_row_in_smem_kernel, (ROW_MAX_C + 3) / 4 * 16);

@@ -445,6 +445,71 @@ def test_repeats_are_equal_to_the_bit(gt, M, V, E):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("M, V, E, K", [(1, 900, 96, 3), (12, 2000, 96, 1), (300, 5003, 104, 1), (300, 5003, 104, 7), (1100, 33001, 40, 5)])
+def test_captured_and_replayed(gt, M, V, E, K):
+    """Forward and backward of a linear loss, and a distillation of given logits with its gradient, captured from the context's
+    stream and replayed on other inputs in the same buffers: the bits of the calls made one by one."""
+    import torch
+
+    lib, ctx = gt.load_library(), gt.context()
+    stream = torch.cuda.ExternalStream(lib.gt_ctx_stream(ctx))
+    mean, prec, T = gt.REDUCTIONS["mean"], gt.PREC_TF32X3, 1.0 if K == 1 else 1.5
+    n_saved, n_scratch, n_given = c_size_t(0), c_size_t(0), c_size_t(0)
+    gt.check(lib.gt_linear_loss_sizes(ctx, M, V, E, K, prec, byref(n_saved), byref(n_scratch)), "sizes")
+    gt.check(lib.gt_topk_distillation_sizes(ctx, M, V, K, byref(n_given)), "sizes")
+
+    def new(*shape, dtype=torch.float32):
+        return torch.zeros(shape, dtype=dtype, device="cuda")
+
+    x, w, ids, teacher, logits = new(M, E), new(V, E), new(M, K), new(M, K), new(M, V)
+    loss, dx, dw, loss_given, dlogits, one = new(1), new(M, E), new(V, E), new(1), new(M, V), torch.ones(1, device="cuda")
+    saved, scratch, given = (new(n.value, dtype=torch.uint8) for n in (n_saved, n_scratch, n_given))
+
+    def run():
+        p = lambda t: c_void_p(t.data_ptr())          # noqa: E731
+        if K == 1:
+            gt.check(lib.gt_linear_cross_entropy(ctx, p(loss), p(saved), p(scratch), p(x), p(w), p(ids), M, V, E, -1.0, mean, prec), "forward")
+        else:
+            gt.check(lib.gt_linear_topk_distillation(ctx, p(loss), p(saved), p(scratch), p(x), p(w), p(ids), p(teacher), M, V, E, K, T, mean, prec),
+                     "forward")
+        gt.check(lib.gt_linear_loss_backward(ctx, p(dx), p(dw), p(saved), p(scratch), p(x), p(w), p(one), M, V, E, K, T, mean, prec, 0, 0), "backward")
+        gt.check(lib.gt_topk_distillation(ctx, p(loss_given), p(given), p(dlogits), V, p(logits), V, p(ids), p(teacher), M, V, K, T, mean), "given")
+
+    def fill(seed):
+        rng = np.random.default_rng([M, V, K, seed])
+        hx, hw = hidden(rng, M, V, E)
+        hi, ht = teacher_of(rng, M, V, K, ragged=False)
+        if M > 1:
+            hi[seed] = -1.0                           # a row without a target, another one each time
+        for t, a in ((x, hx), (w, hw), (ids, hi), (teacher, ht), (logits, rng.standard_normal((M, V)).astype(np.float32))):
+            t.copy_(torch.from_numpy(a))
+        torch.cuda.synchronize()
+
+    def results():
+        torch.cuda.synchronize()
+        return [t.clone().cpu().numpy() for t in (loss, dx, dw, loss_given, dlogits)]
+
+    want = []
+    for seed in (1, 2):
+        fill(seed)
+        run()
+        want.append(results())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        run()
+    for seed in (1, 2, 1):
+        fill(seed)
+        for t in (loss, dx, dw, loss_given, dlogits):
+            t.fill_(np.nan)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+        for got, wanted in zip(results(), want[seed - 1]):
+            assert np.array_equal(got, wanted)
+    gt.device_status()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("M, V, E", [(8192, 12800, 64), (2500, 40000, 130)])
 def test_many_pieces_against_the_path_through_the_logits(gt, monkeypatch, M, V, E):
     """Several pieces of the vocabulary, dx of each added to the last: against linear_tied and cross_entropy, whose products are
